@@ -1,0 +1,594 @@
+"""The operators of a serving step over a paged 8-bit K/V cache, as cases that can be timed and checked.
+
+`run` computes each in its plain form with elementary torch operations, or, where `own` is set, by
+the calls that a host program makes of this repository's kernels.  `exact` restates them in 64 bits.
+
+Kinds of case and the fields they take:
+
+  append  seqs, rows_lo, rows_hi, past_lo, past_hi, page, heads, kv_heads, head_dim, rotary, k_eq_v
+          q/k norm, rotary position and the 8-bit paged cache write of every row of a batch
+  attn    seqs, rows_lo, rows_hi, past_lo, past_hi, page, heads, kv_heads, head_dim, window, unscaled
+          attention of the batch's rows over the cache (window 0: over all of it)
+  probs   rows, vocab, cap, temperature
+          logits to probabilities
+  verify  seqs, draft, vocab, draft_probs
+          drafted tokens against the target's probabilities
+
+A sequence's rows and past tokens lie between lo and hi, spread evenly.  A cache page holds `page`
+tokens in blocks of 16; a block of one kv head has one scale, a power of two.  Codes lie as
+K [page][head][block][dim / 16][16 tokens][16 dims] and V [page][head][block][4][dim][4 tokens].
+"""
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+_EPS = 1e-6
+_THETA = 10000.0
+_BLOCK = 16
+
+
+def listed():
+    heads = dict(heads=16, kv_heads=8, head_dim=256)  # the 12B layer of the repository's benchmark
+    return [
+        # One generated token of one chat: launches and one memory round trip.
+        dict(name="append_1", kind="append", seqs=1, rows_lo=1, rows_hi=1, past_lo=543, past_hi=543, page=16,
+             rotary=256, k_eq_v=False, **heads),
+        # A serving step: sequences with a token or a few drafted ones each.
+        dict(name="append_32_ragged", kind="append", seqs=32, rows_lo=1, rows_hi=9, past_lo=20, past_hi=4000,
+             page=32, rotary=256, k_eq_v=False, **heads),
+        # A long prompt in one call, with a quarter of the dims rotated as the full layers do.
+        dict(name="append_prompt_2000", kind="append", seqs=1, rows_lo=2000, rows_hi=2000, past_lo=0, past_hi=0,
+             page=64, rotary=64, k_eq_v=False, **heads),
+        # The attention of one generated token of one chat, unscaled scores as the engine has them.
+        dict(name="attn_1x544", kind="attn", seqs=1, rows_lo=1, rows_hi=1, past_lo=543, past_hi=543, page=16,
+             window=0, unscaled=True, **heads),
+        # A serving step of ragged sequences, a token each.
+        dict(name="attn_32_ragged", kind="attn", seqs=32, rows_lo=1, rows_hi=1, past_lo=20, past_hi=4000, page=32,
+             window=0, unscaled=False, **heads),
+        # Drafted tokens of a few sequences, verified in one pass.
+        dict(name="attn_8x5_drafts", kind="attn", seqs=8, rows_lo=5, rows_hi=5, past_lo=1000, past_hi=3000, page=32,
+             window=0, unscaled=False, **heads),
+        # One token at the end of a very long document.
+        dict(name="attn_1x120000", kind="attn", seqs=1, rows_lo=1, rows_hi=1, past_lo=119999, past_hi=119999, page=64,
+             window=0, unscaled=False, **heads),
+        # A prompt's rows over their own keys.
+        dict(name="attn_prompt_2000", kind="attn", seqs=1, rows_lo=2000, rows_hi=2000, past_lo=0, past_hi=0, page=64,
+             window=0, unscaled=False, **heads),
+        # The vocabulary of the repository's benchmark: one sampled token; the rows of a drafted batch.
+        dict(name="probs_1", kind="probs", rows=1, vocab=262144, cap=30.0, temperature=0.8),
+        dict(name="probs_40", kind="probs", rows=40, vocab=262144, cap=30.0, temperature=0.8),
+        # Drafts without probabilities (looked up in the text) of one chat; a drafting model's of a batch.
+        dict(name="verify_1", kind="verify", seqs=1, draft=4, vocab=262144, draft_probs=False),
+        dict(name="verify_32", kind="verify", seqs=32, draft=5, vocab=262144, draft_probs=True),
+    ]
+
+
+def _between(rng, lo, hi):
+    """A whole number from lo to hi, even over its logarithm."""
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["append", "append", "attn", "attn", "attn", "attn", "probs", "verify"])
+    if kind == "probs":
+        return dict(kind=kind, rows=_between(rng, 1, 40), vocab=_between(rng, 1000, 262144), cap=rng.choice([0.0, 30.0]),
+                    temperature=rng.choice([0.5, 0.8, 1.0, 1.5]))
+    if kind == "verify":
+        return dict(kind=kind, seqs=_between(rng, 1, 32), draft=rng.randint(1, 5), vocab=_between(rng, 1000, 262144),
+                    draft_probs=rng.choice([True, True, False]))
+    heads, kv_heads, head_dim = rng.choice([(16, 8, 256), (16, 8, 256), (16, 8, 128), (8, 8, 64), (16, 4, 256), (8, 1, 256),
+                                            (12, 4, 96), (8, 2, 512)])
+    case = dict(kind=kind, page=rng.choice([16, 32, 64, 128]), heads=heads, kv_heads=kv_heads, head_dim=head_dim)
+    shape = rng.choice(["token", "tokens", "drafts", "prompt", "chunk"])
+    if shape == "token":
+        case.update(seqs=1, rows_lo=1, rows_hi=1, past_lo=_between(rng, 1, 60000))
+    elif shape == "tokens":
+        case.update(seqs=rng.randint(2, 32), rows_lo=1, rows_hi=1, past_lo=rng.randint(0, 100))
+        case.update(past_hi=_between(rng, 100, 4000))
+    elif shape == "drafts":
+        rows = rng.randint(2, 9)
+        case.update(seqs=rng.randint(1, 8), rows_lo=rng.randint(1, rows), rows_hi=rows, past_lo=rng.randint(0, 500))
+        case.update(past_hi=_between(rng, 500, 4000))
+    elif shape == "prompt":
+        case.update(seqs=1, rows_lo=_between(rng, 16, 1900), past_lo=0)
+    else:  # a prompt's later part, or a few short prompts
+        seqs = rng.randint(1, 4)
+        rows = _between(rng, 16, 1000 // seqs)
+        case.update(seqs=seqs, rows_lo=rng.randint(1, rows), rows_hi=rows, past_lo=rng.randint(0, 800))
+    case.setdefault("rows_hi", case["rows_lo"])
+    case.setdefault("past_hi", case["past_lo"])
+    if kind == "append":
+        case.update(rotary=rng.choice([head_dim, head_dim // 4, head_dim // 2]), k_eq_v=rng.choice([False, False, True]))
+    else:
+        case.update(window=rng.choice([0, 0, 512, _between(rng, 1, 2000)]), unscaled=rng.choice([False, False, True]))
+    return case
+
+
+# ---- inputs ----------------------------------------------------------------------------------
+def _generator(seed, stream):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(int(seed) * 1009 + stream)
+    return g
+
+
+def _normal(seed, stream, shape, std=1.0, mean=0.0):
+    return torch.randn(shape, generator=_generator(seed, stream), device="cuda") * std + mean
+
+
+def _uniform(seed, stream, shape):
+    return torch.rand(shape, generator=_generator(seed, stream), device="cuda")
+
+
+def _spread(lo, hi, n, step):
+    """n numbers from lo to hi, evenly spread, in an order that is not sorted."""
+    return [lo + (hi - lo) * ((i * step) % n) // max(1, n - 1) for i in range(n)]
+
+
+def _lengths(case):
+    """Rows and past tokens of each sequence."""
+    n = case["seqs"]
+    return _spread(case["rows_lo"], case["rows_hi"], n, 3 if n % 3 else 1), _spread(case["past_lo"], case["past_hi"], n, 5 if n % 5 else 1)
+
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _two_to(e, dtype):
+    """2^e by its bits."""
+    if dtype == torch.float64:
+        return ((e.long() + 1023) << 52).view(torch.float64)
+    return ((e.int() + 127) << 23).view(torch.float32)
+
+
+def _blocks_of(values):
+    """The codes and scales of [..., tokens, dims] with the tokens in blocks of 16: powers of two."""
+    x = values.unflatten(-2, (-1, _BLOCK))
+    amax = x.abs().amax((-2, -1))
+    m, e = torch.frexp(amax / 127.0)
+    e = torch.where(m == 0.5, e - 1, e)
+    scale = torch.where(amax > 0, _two_to(e, amax.dtype), torch.zeros_like(amax))
+    codes = torch.round(x / torch.where(scale > 0, scale, torch.ones_like(scale))[..., None, None])
+    return codes.to(torch.int8), scale
+
+
+def _k_laid(codes):
+    """[page][head][block][16 tokens][dims] as the cache holds keys."""
+    return codes.unflatten(-1, (-1, 16)).transpose(-2, -3).contiguous()
+
+
+def _v_laid(codes):
+    return codes.unflatten(-2, (4, 4)).transpose(-1, -2).contiguous()
+
+
+def _k_rows(k):
+    """The same back: [page][head][token][dim]."""
+    return k.transpose(-2, -3).flatten(-2, -1).flatten(-3, -2)
+
+
+def _v_rows(v):
+    return v.transpose(-1, -2).flatten(-3, -2).flatten(-3, -2)
+
+
+def _paged(case, seed):
+    """A batch over a cache with something in every page, in no order."""
+    rows, past = _lengths(case)
+    page, H, D = case["page"], case["kv_heads"], case["head_dim"]
+    per = max(-(-(r + p) // page) for r, p in zip(rows, past))
+    order = torch.randperm(len(rows) * per, generator=_generator(seed, 90), device="cuda")
+    start = np.concatenate([[0], np.cumsum(rows)])
+    k, ks = _blocks_of(_normal(seed, 91, (len(rows) * per, H, page, D)))
+    k = _k_laid(k)
+    v, vs = _blocks_of(_normal(seed, 92, (len(rows) * per, H, page, D)))
+    v = _v_laid(v)
+    return dict(case=dict(case), rows=rows, past=past, total=int(start[-1]), most=max(rows), reach=max(r + p for r, p in zip(rows, past)),
+                seq_start=_ints(start.tolist()), past_len=_ints(past), pages=order.reshape(len(rows), per).to(torch.int32),
+                k=k, v=v, k_scale=ks, v_scale=vs)
+
+
+def _append_inputs(case, seed):
+    nq, H, D = case["heads"], case["kv_heads"], case["head_dim"]
+    total = sum(_lengths(case)[0])
+    qkv = _normal(seed, 1, (total, (nq + 2 * H) * D))  # the packed rows of one projection
+    return dict(qkv=qkv, q_norm=_normal(seed, 2, (D,), 0.1, 1.0), k_norm=_normal(seed, 3, (D,), 0.1, 1.0))
+
+
+def _logits(case, seed):
+    return _normal(seed, 1, (case["rows"], case["vocab"]), 3.0)
+
+
+def _drafted(case, seed):
+    B, n, V = case["seqs"], case["draft"], case["vocab"]
+    z = _normal(seed, 1, (B, n + 1, V), 3.0)
+    p = torch.softmax(z, -1)
+    zq = z[:, :n] + _normal(seed, 2, (B, n, V), 0.6)
+    if case["draft_probs"]:
+        q = torch.softmax(zq, -1)
+        g = -torch.log(-torch.log(_uniform(seed, 3, (B, n, V)).clamp(1e-9, 1 - 1e-7)))
+        token = (zq + g).argmax(-1)
+    else:
+        q, token = None, zq.argmax(-1)
+    some = torch.randint(max(0, n - 1), n + 1, (B,), generator=_generator(seed, 4), device="cuda")
+    return dict(p=p, q=q, token=token.to(torch.int32), drafted=some.to(torch.int32), u=_uniform(seed, 5, (B, n)), pick=_uniform(seed, 6, (B,)))
+
+
+def prepare(case, seed):
+    kind = case["kind"]
+    if kind == "probs":
+        return dict(case=dict(case), logits=_logits(case, seed))
+    if kind == "verify":
+        return dict(case=dict(case), **_drafted(case, seed))
+    s = _paged(case, seed)
+    if kind == "append":
+        s.update(_append_inputs(case, seed))
+        # what the call may change, read back: every row from the start of each sequence's first block
+        first = [p - p % _BLOCK for p in s["past"]]
+        s["read_rows"] = [p - f + r for p, f, r in zip(s["past"], first, s["rows"])]
+        s["read_start"] = _ints(np.concatenate([[0], np.cumsum(s["read_rows"])]).tolist())
+        s["read_past"] = _ints(first)
+    else:
+        s["q"] = _normal(seed, 1, (s["total"], case["heads"] * case["head_dim"]))
+    return s
+
+
+# ---- the plain forms -------------------------------------------------------------------------
+def _row_places(start, past, total):
+    """Sequence and position of each of a batch's rows."""
+    row = torch.arange(total, device="cuda")
+    seq = torch.searchsorted(start[1:].long(), row, right=True)
+    return seq, past.long()[seq] + row - start.long()[seq]
+
+
+def _rope(x, position, rotary):
+    """[rows][heads][dims]; the first rotary dims turn in split halves, by angles in 64 bits."""
+    half = rotary // 2
+    a = position.double()[:, None] * torch.pow(_THETA, torch.arange(half, dtype=torch.float64, device="cuda") * (-2.0 / rotary))
+    c, s = torch.cos(a)[:, None].to(x.dtype), torch.sin(a)[:, None].to(x.dtype)
+    u, v = x[..., :half], x[..., half:rotary]
+    return torch.cat([u * c - v * s, u * s + v * c, x[..., rotary:]], -1)
+
+
+def _rms(x):
+    return x / torch.sqrt((x * x).mean(-1, keepdim=True) + _EPS)
+
+
+def _power(amax):
+    """The least power of two whose 127-fold reaches amax; 0 for 0 (64 bits)."""
+    m, e = torch.frexp(amax / 127.0)
+    e = torch.where((m == 0.5) & (127.0 * _two_to(e - 1, amax.dtype) >= amax), e - 1, e)
+    return torch.where(amax > 0, _two_to(e, amax.dtype), torch.zeros_like(amax))
+
+
+def _write(codes, scales, rows_of, laid, x, page, block, within):
+    """Puts x [rows][heads][dims] (64 bits) into the blocks, growing their scales; codes and scales in place."""
+    nb = codes.shape[2]
+    H, D = x.shape[1:]
+    place, inverse = torch.unique(page * nb + block, return_inverse=True)
+    first = torch.full((place.numel(),), _BLOCK, device="cuda").scatter_reduce(0, inverse, within, "amin")
+    amax = torch.zeros(place.numel(), H, dtype=torch.float64, device="cuda")
+    amax = amax.scatter_reduce(0, inverse[:, None].expand(-1, H), x.abs().amax(-1), "amax")
+    at, blk = place // nb, place % nb
+    old = torch.where(first[:, None] > 0, scales[at, :, blk].double(), 0.0)
+    new = torch.maximum(old, _power(amax))
+    some = torch.where(new > 0, new, 1.0)
+    held = rows_of(codes[at, :, blk][:, :, None]).double()  # [place][head][16][dim]
+    held = torch.round(held * (old / some)[..., None, None])
+    held[inverse, :, within] = torch.round(x / some[inverse][..., None])
+    codes[at, :, blk] = laid(held.to(torch.int8)[:, :, None])[:, :, 0]
+    scales[at, :, blk] = new.float()
+
+
+def _plain_append(s):
+    case = s["case"]
+    nq, H, D, page = case["heads"], case["kv_heads"], case["head_dim"], case["page"]
+    seq, position = _row_places(s["seq_start"], s["past_len"], s["total"])
+    q, k, v = (t.unflatten(-1, (-1, D)) for t in s["qkv"].split([nq * D, H * D, H * D], -1))
+    q = _rope(_rms(q) * s["q_norm"], position, case["rotary"])
+    # a code is decided next to a border: keys and values in 64 bits
+    v = _rms(k.double() if case["k_eq_v"] else v.double())
+    k = _rope(_rms(k.double()) * s["k_norm"].double(), position, case["rotary"])
+    at = s["pages"].long()[seq, position // page]
+    block, within = position % page // _BLOCK, position % _BLOCK
+    _write(s["k"], s["k_scale"], _k_rows, _k_laid, k, at, block, within)
+    _write(s["v"], s["v_scale"], _v_rows, _v_laid, v, at, block, within)
+    seq, position = _row_places(s["read_start"], s["read_past"], sum(s["read_rows"]))
+    at, block, within = s["pages"].long()[seq, position // page], position % page // _BLOCK, position % _BLOCK
+    k = s["k"][at, :, block, :, within].flatten(-2).float() * s["k_scale"][at, :, block][..., None]
+    v = s["v"][at, :, block, within // 4, :, within % 4].float() * s["v_scale"][at, :, block][..., None]
+    return {"q": q.flatten(1), "k": k.flatten(1), "v": v.flatten(1)}
+
+
+def _dense(s, dtype):
+    """Keys and values of each sequence in a row: [seq][head][token][dim]."""
+    at = s["pages"].long()
+
+    def gathered(codes, scale, rows_of):
+        x = rows_of(codes[at].to(dtype) * scale[at].to(dtype)[..., None, None, None])  # [seq][page][head][token][dim]
+        return x.transpose(1, 2).flatten(2, 3)
+
+    return gathered(s["k"], s["k_scale"], _k_rows), gathered(s["v"], s["v_scale"], _v_rows)
+
+
+def _plain_attn(s):
+    case = s["case"]
+    nq, H, D = case["heads"], case["kv_heads"], case["head_dim"]
+    B, T, G = case["seqs"], s["most"], nq // H
+    scale = 1.0 if case["unscaled"] else D ** -0.5
+    k, v = _dense(s, torch.float32)
+    seq, position = _row_places(s["seq_start"], s["past_len"], s["total"])
+    row = position - s["past_len"].long()[seq]
+    q = torch.zeros(B, T, nq, D, device="cuda")
+    q[seq, row] = s["q"].unflatten(-1, (nq, D))
+    q = q.reshape(B, T, H, G, D).transpose(1, 2).reshape(B, H, T * G, D)
+    scores = torch.matmul(q, k.transpose(-1, -2).contiguous()) * scale
+    token = torch.arange(k.shape[2], device="cuda")
+    own_position = s["past_len"].long()[:, None] + torch.arange(T, device="cuda")
+    seen = token <= own_position[..., None]
+    if case["window"]:
+        seen &= token > own_position[..., None] - case["window"]
+    scores = scores.masked_fill(~seen.repeat_interleave(G, 1)[:, None], -math.inf)
+    e = torch.exp(scores - scores.amax(-1, keepdim=True))
+    out = torch.matmul(e, v) / e.sum(-1, keepdim=True)
+    out = out.reshape(B, H, T, G, D).transpose(1, 2).reshape(B, T, nq * D)
+    return out[seq, row]
+
+
+def _plain_probs(s):
+    x = s["logits"]
+    if s["case"]["cap"]:
+        x = s["case"]["cap"] * torch.tanh(x / s["case"]["cap"])
+    x = x / s["case"]["temperature"]
+    e = torch.exp(x - x.amax(-1, keepdim=True))
+    return e / e.sum(-1, keepdim=True)
+
+
+def _plain_verify(s):
+    p, q, token, drafted = s["p"], s["q"], s["token"], s["drafted"].long()
+    B, n = token.shape
+    seq, slot = torch.arange(B, device="cuda"), torch.arange(n + 1, device="cuda")
+    pt = p[:, :n].gather(2, token.long()[..., None])[..., 0].double()
+    qt = q.gather(2, token.long()[..., None])[..., 0].double() if q is not None else torch.ones_like(pt)
+    fine = (s["u"].double() * qt < pt) & (slot[:n] < drafted[:, None])
+    kept = torch.cumprod(fine.long(), 1).sum(1)
+    stop = kept.clamp(max=n - 1)
+    target = p[seq, kept].double()
+    if q is not None:
+        other = q[seq, stop].double()
+    else:
+        other = torch.zeros_like(target).scatter(1, token[seq, stop].long()[:, None], 1.0)
+    weight = torch.clamp(target - torch.where((kept < drafted)[:, None], other, 0.0), min=0.0)
+    weight = torch.where(weight.sum(1, keepdim=True) > 0, weight, target)
+    reached = torch.cumsum(weight, 1)
+    hit = reached > s["pick"].double()[:, None] * reached[:, -1:]
+    chosen = hit.long().argmax(1).to(torch.int32)
+    padded = torch.cat([token, torch.full((B, 1), -1, dtype=torch.int32, device="cuda")], 1)
+    tokens = torch.where(slot < kept[:, None], padded, torch.where(slot == kept[:, None], chosen[:, None], -1))
+    return {"tokens": tokens, "accepted": kept.to(torch.int32)}
+
+
+# ---- the same by the framework's calls -------------------------------------------------------
+_ctx = None
+
+
+def _binding():
+    """The binding and its context (one per process, as a host has it)."""
+    global _ctx
+    import importlib
+    import os
+    import sys
+    where = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ai-research_amd")
+    if where not in sys.path:
+        sys.path.insert(0, where)
+    gh = importlib.import_module("gemma_hip")
+    if _ctx is None:
+        _ctx = gh.Context()
+    return gh, _ctx
+
+
+def _f32(*shape):
+    return torch.empty(shape, device="cuda")
+
+
+def _i32(*shape):
+    return torch.empty(shape, dtype=torch.int32, device="cuda")
+
+
+def _handles(s):
+    """What a host makes once for a state: descriptors, result buffers and workspace."""
+    gh, ctx = _binding()
+    case, kind = s["case"], s["case"]["kind"]
+    p = lambda t: t.data_ptr()  # noqa: E731
+    h = dict(ctx=ctx)
+    if kind == "probs":
+        h["out"] = _f32(case["rows"], case["vocab"])
+        h["bytes"] = ctx.logit_probs_workspace(case["rows"], case["vocab"])
+    elif kind == "verify":
+        h["out"] = dict(tokens=_i32(case["seqs"], case["draft"] + 1), accepted=_i32(case["seqs"]))
+        h["bytes"] = ctx.spec_verify_workspace(case["seqs"], case["vocab"])
+    else:
+        h["cache"] = gh.Kv8Cache(p(s["k"]), p(s["v"]), p(s["k_scale"]), p(s["v_scale"]), s["k"].shape[0], case["page"],
+                                 case["kv_heads"], case["head_dim"])
+        h["batch"] = gh.Kv8Batch(p(s["seq_start"]), p(s["past_len"]), p(s["pages"]), case["seqs"], s["pages"].shape[1],
+                                 s["total"], s["most"])
+        width = case["heads"] * case["head_dim"]
+        if kind == "append":
+            back, kv = sum(s["read_rows"]), case["kv_heads"] * case["head_dim"]
+            h["out"] = dict(q=_f32(s["total"], width), k=_f32(back, kv), v=_f32(back, kv))
+            h["read"] = gh.Kv8Batch(p(s["read_start"]), p(s["read_past"]), p(s["pages"]), case["seqs"], s["pages"].shape[1],
+                                    back, max(s["read_rows"]))
+        else:
+            h["out"] = _f32(s["total"], width)
+            h["bytes"] = ctx.kv8_attn_workspace(h["cache"], h["batch"], case["heads"], case["window"], s["reach"])
+    if h.get("bytes"):
+        h["work"] = torch.empty(h["bytes"], dtype=torch.uint8, device="cuda")
+    return h
+
+
+def _run_own(s):
+    if "handles" not in s:
+        s["handles"] = _handles(s)
+    h, case, kind = s["handles"], s["case"], s["case"]["kind"]
+    p = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    ctx, out, work, size = h["ctx"], h["out"], p(h.get("work")), h.get("bytes", 0)
+    if kind == "probs":
+        ctx.logit_probs(p(s["logits"]), p(out), case["rows"], case["vocab"], case["vocab"], case["cap"], case["temperature"], work, size)
+    elif kind == "verify":
+        ctx.spec_verify(p(s["p"]), p(s["q"]), p(s["token"]), p(s["drafted"]), p(s["u"]), p(s["pick"]), p(out["tokens"]),
+                        p(out["accepted"]), case["seqs"], case["draft"], case["vocab"], work, size)
+    elif kind == "append":
+        nq, H, D = case["heads"], case["kv_heads"], case["head_dim"]
+        width, row = (nq + 2 * H) * D, p(s["qkv"])
+        ctx.kv8_append(h["cache"], h["batch"], row, row + 4 * nq * D, row + 4 * (nq + H) * D, width, width, p(s["q_norm"]),
+                       p(s["k_norm"]), p(out["q"]), nq, case["rotary"], case["k_eq_v"], _THETA, _EPS)
+        ctx.kv8_read(h["cache"], h["read"], p(out["k"]), p(out["v"]))
+    else:
+        scale = 1.0 if case["unscaled"] else case["head_dim"] ** -0.5
+        ctx.kv8_attn(h["cache"], h["batch"], p(s["q"]), p(out), case["heads"], scale, case["window"], s["reach"], work, size)
+    return out
+
+
+def run(state):
+    if own:
+        return _run_own(state)
+    return {"append": _plain_append, "attn": _plain_attn, "probs": _plain_probs, "verify": _plain_verify}[state["case"]["kind"]](state)
+
+
+# ---- what a pass cannot do without -----------------------------------------------------------
+def work(case):
+    kind = case["kind"]
+    if kind == "probs":
+        return {"bytes": 8 * case["rows"] * case["vocab"], "flops": 8 * case["rows"] * case["vocab"]}
+    if kind == "verify":
+        rows = 2 if case["draft_probs"] else 1  # the row where a sequence stops
+        return {"bytes": 4 * rows * case["seqs"] * case["vocab"], "flops": 2 * case["seqs"] * case["vocab"]}
+    rows, past = _lengths(case)
+    nq, H, D = case["heads"], case["kv_heads"], case["head_dim"]
+    if kind == "append":
+        back = sum(p % _BLOCK + r for r, p in zip(rows, past))
+        n = sum(rows)
+        kv = (1 if case["k_eq_v"] else 2) * H
+        return {"bytes": 4 * n * (2 * nq + kv) * D + 2 * n * H * D + 2 * back * H * D * 5, "flops": 8 * n * (nq + 2 * H) * D}
+    window = case["window"] or 1 << 40
+    read = sum(min(r + p, r + window - 1) for r, p in zip(rows, past))
+    pairs = sum(min(p + i + 1, window) for r, p in zip(rows, past) for i in range(r))
+    return {"bytes": read * H * (2 * D + 8 / _BLOCK) + 8 * sum(rows) * nq * D, "flops": 4 * pairs * nq * D}
+
+
+# ---- the same in 64 bits ---------------------------------------------------------------------
+def _turned(x, position, rotary):
+    """x [heads][dims] of one position as complex numbers times e^(i angle)."""
+    half = rotary // 2
+    a = position * _THETA ** (-2.0 * np.arange(half) / rotary)
+    z = (x[:, :half] + 1j * x[:, half:rotary]) * np.exp(1j * a)
+    return np.concatenate([z.real, z.imag, x[:, rotary:]], 1)
+
+
+def _code(block_scale, x):
+    return np.rint(x / block_scale) if block_scale > 0 else np.zeros_like(x)
+
+
+def _exact_append(case, seed):
+    s = _paged(case, seed)
+    s.update({k: v.double().cpu().numpy() for k, v in _append_inputs(case, seed).items()})
+    nq, H, D, page = case["heads"], case["kv_heads"], case["head_dim"], case["page"]
+    if s["total"] > 20000:
+        return None
+    pages = s["pages"].cpu().numpy()
+    codes = {"k": _k_rows(s["k"]), "v": _v_rows(s["v"])}
+    q_all, k_all, v_all = [], [], []
+    at = 0
+    for b, (rows, past) in enumerate(zip(s["rows"], s["past"])):
+        first = past - past % _BLOCK
+        x = s["qkv"][at:at + rows].reshape(rows, nq + 2 * H, D)
+        at += rows
+        x = x / np.sqrt((x * x).mean(-1, keepdims=True) + _EPS)
+        v = x[:, nq:nq + H] if case["k_eq_v"] else x[:, nq + H:]
+        q = np.stack([_turned(x[i, :nq] * s["q_norm"], past + i, case["rotary"]) for i in range(rows)])
+        k = np.stack([_turned(x[i, nq:nq + H] * s["k_norm"], past + i, case["rotary"]) for i in range(rows)])
+        q_all.append(q.reshape(rows, -1))
+        for name, new, gather in (("k", k, k_all), ("v", v, v_all)):
+            for start in range(first, past + rows, _BLOCK):
+                held = min(_BLOCK, max(0, past - start))
+                fresh = new[max(0, start - past):max(0, start - past) + _BLOCK - held]
+                where, block = pages[b, start // page], start % page // _BLOCK
+                old = s[name + "_scale"][where, :, block].double().cpu().numpy()
+                lines = codes[name][where, :, block * _BLOCK:block * _BLOCK + held].double().cpu().numpy()
+                out = np.zeros((held + len(fresh), H, D))
+                for h in range(H):
+                    most = np.abs(fresh[:, h]).max()
+                    size = 2.0 ** math.ceil(math.log2(most / 127.0)) if most > 0 else 0.0
+                    if most > 0 and size / 2 * 127 >= most:
+                        size /= 2
+                    if size * 127 < most:
+                        size *= 2
+                    size = max(size, old[h] if held else 0.0)
+                    if held and size > 0:
+                        out[:held, h] = np.rint(lines[h] * old[h] / size) * size
+                    out[held:, h] = _code(size, fresh[:, h]) * size
+                gather.append(out.reshape(len(out), -1))
+    as_tensor = lambda v: torch.from_numpy(np.concatenate(v))  # noqa: E731
+    return {"q": as_tensor(q_all), "k": as_tensor(k_all), "v": as_tensor(v_all)}
+
+
+def _exact_attn(case, seed):
+    s = prepare(case, seed)
+    nq, H, D, page = case["heads"], case["kv_heads"], case["head_dim"], case["page"]
+    G, at, out = nq // H, 0, []
+    for b, (rows, past) in enumerate(zip(s["rows"], s["past"])):
+        n = past + rows
+        held = s["pages"][b, :-(-n // page)].long()
+        k, v = ((rows_of(c[held].double()) * sc[held].double().repeat_interleave(_BLOCK, -1)[..., None]).transpose(0, 1).flatten(1, 2)[:, :n]
+                for c, sc, rows_of in ((s["k"], s["k_scale"], _k_rows), (s["v"], s["v_scale"], _v_rows)))
+        q = s["q"][at:at + rows].double().reshape(rows, H, G, D)
+        at += rows
+        token, mine = torch.arange(n, device="cuda"), past + torch.arange(rows, device="cuda")
+        hidden = token[None] > mine[:, None]
+        if case["window"]:
+            hidden |= token[None] <= mine[:, None] - case["window"]
+        heads = []
+        for h in range(H):
+            score = (q[:, h].reshape(rows * G, D) @ k[h].T).reshape(rows, G, n)
+            if not case["unscaled"]:
+                score = score / math.sqrt(D)
+            heads.append(torch.softmax(score.masked_fill(hidden[:, None], -math.inf), -1).reshape(rows * G, n) @ v[h])
+        out.append(torch.stack(heads).reshape(H, rows, G, D).transpose(0, 1).reshape(rows, nq * D))
+    return torch.cat(out)
+
+
+def _exact_verify(case, seed):
+    s = {k: v.cpu().numpy() for k, v in _drafted(case, seed).items() if v is not None}
+    tokens = np.full((case["seqs"], case["draft"] + 1), -1, np.int32)
+    accepted = np.zeros(case["seqs"], np.int32)
+    for b in range(case["seqs"]):
+        i, w = 0, None
+        while w is None:
+            w = s["p"][b, i].astype(np.float64)
+            if i < s["drafted"][b]:
+                x = s["token"][b, i]
+                q = s["q"][b, i].astype(np.float64) if "q" in s else np.eye(1, case["vocab"], x)[0]
+                if float(s["u"][b, i]) * q[x] < w[x]:
+                    tokens[b, i], w = x, None
+                    i += 1
+                else:
+                    rest = np.maximum(w - q, 0.0)
+                    w = rest if rest.any() else w
+        total = np.cumsum(w)
+        tokens[b, i], accepted[b] = np.searchsorted(total, float(s["pick"][b]) * total[-1], "right"), i
+    return {"tokens": torch.from_numpy(tokens), "accepted": torch.from_numpy(accepted)}
+
+
+def exact(case, seed):
+    kind = case["kind"]
+    if kind == "append":
+        return _exact_append(case, seed)
+    if kind == "attn":
+        return _exact_attn(case, seed)
+    if kind == "verify":
+        return _exact_verify(case, seed)
+    x = _logits(case, seed).double()
+    if case["cap"]:
+        x = torch.tanh(x / case["cap"]) * case["cap"]
+    return torch.softmax(x / case["temperature"], -1)
