@@ -23,13 +23,13 @@ DEVICE_FLAGS = ["--offload-arch=gfx950", "--genco", "--no-gpu-bundle-output", "-
                 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                 "-I", CSRC, "-I", os.path.join(ROOT, "include")]
 
-KERNEL_FAMILIES = ["gemv", "gemv_norm", "util", "attn", "norm", "prefill"]
+KERNEL_FAMILIES = ["gemv", "gemv_norm", "util", "attn", "norm", "prefill", "kv8", "sample"]
 
 # Per-family extra flags.  The prefill GEMMs scale each 32-block's MFMA sum on
 # the VALU; in VGPR form the MFMA results need no v_accvgpr_read first.
 FAMILY_FLAGS = {"prefill": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
-HOST_SOURCES = ["runtime.cpp", "engine.cpp", "model.cpp", "ring.cpp"]
+HOST_SOURCES = ["runtime.cpp", "engine.cpp", "model.cpp", "ring.cpp", "serving.cpp"]
 HIP_HOST_SOURCES = ["noalloc.hip"]
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-pthread", "-ffp-contract=off",
               "-Wall", "-Wno-unused-result", "-D__HIP_PLATFORM_AMD__",

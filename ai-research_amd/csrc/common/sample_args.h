@@ -1,0 +1,24 @@
+// sample_args.h -- argument blocks of the sampling kernels (sample.hip), shared
+// with the host launcher (passed by value).
+#pragma once
+#include <stdint.h>
+
+#define SAMPLE_CHUNK 4096u  // elements of a row that one workgroup takes
+
+struct ProbsArgs {
+  const float* logits;
+  float* probs;
+  float* part;  // [row][chunk] {max, sum}
+  uint64_t stride;
+  uint32_t vocab, chunks;
+  float cap, mul;  // soft-cap (0: none); log2(e) / temperature
+};
+
+struct VerifyArgs {
+  const float *target, *draft;  // [seq][max_draft + 1][vocab], [seq][max_draft][vocab] or null
+  const uint32_t *tokens, *n_draft;
+  const float *u, *pick;
+  uint32_t *out, *accepted;
+  double* part;  // [seq][chunk] {weights left, target}
+  uint32_t max_draft, vocab, chunks;
+};

@@ -1,0 +1,711 @@
+// kv8.hip -- the paged 8-bit K/V cache: append (per-head RMSNorm, rotary
+// positions, quantization, cache write), read-back, and attention, for gfx950.
+//
+// A page holds page_tokens tokens of every kv head; 16 tokens of a head are a
+// block with one scale for its keys and one for its values, a power of two
+// 2^e with the least e for which the block's largest magnitude is <= 127 2^e.
+// Powers of two because a block's scale grows as tokens are appended to it: the
+// codes already there are then shifted (one more rounding, of at most half a
+// step), a value code * 2^e is exact in every float type, and the scales enter
+// products without a rounding.  They cost up to one of the 8 bits.
+//
+// Codes lie as the matrix instructions take them:
+//   K block [D / 16][16 tokens][16 dims]: a lane's 16 bytes are the A operand of
+//     v_mfma_i32_16x16x64_i8 (row = token, 16 dims of the sum) as loaded;
+//   V block [4 groups][D][4 tokens]: a lane's 16 bytes are 4 tokens of 4 dims;
+//     the sum of the second product runs over tokens, in a lane.
+// Either way a wave's load is 1 KB in a row.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../common/kv8_args.h"
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+namespace {
+
+// First row and number of rows of sequence s, whatever seq_start holds.
+__device__ __forceinline__ uint32_t seq_rows(const Kv8Rows& b, uint32_t s, uint32_t* first) {
+  const uint32_t r0 = min(b.seq_start[s], b.num_rows), r1 = min(b.seq_start[s + 1], b.num_rows);
+  *first = r0;
+  return r1 > r0 ? min(r1 - r0, b.max_rows) : 0u;
+}
+
+// The page of block `blk` of sequence s, or num_pages where there is none (past
+// the table's end, or an entry that names no page).
+__device__ __forceinline__ uint32_t page_of(const Kv8View& c, const Kv8Rows& b, uint32_t s, uint64_t blk) {
+  const uint64_t i = blk >> (c.page_shift - 4);
+  if (i >= b.max_pages) return c.num_pages;
+  return min(b.pages[(uint64_t)s * b.max_pages + i], c.num_pages);
+}
+
+// Index of (page, head, block) among the cache's blocks.
+__device__ __forceinline__ uint64_t block_at(const Kv8View& c, uint32_t page, uint32_t head, uint64_t blk) {
+  const uint32_t sh = c.page_shift - 4;
+  return (((uint64_t)page * c.nkv + head) << sh) + (blk & ((1u << sh) - 1u));
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+__device__ __forceinline__ double wave_max(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = fmax(v, __shfl_xor(v, off, 64));
+  return v;
+}
+
+// Dims of pair i < D / 2 of a head: (i, i + rot / 2) for the rotated ones, the
+// others' halves after them.
+__device__ __forceinline__ void pair_dims(uint32_t i, uint32_t D, uint32_t rot, uint32_t* d0, uint32_t* d1) {
+  const uint32_t half = rot / 2;
+  *d0 = i < half ? i : rot + (i - half);
+  *d1 = *d0 + (i < half ? half : (D - rot) / 2);
+}
+
+// ---------------------------------------------------------------------------
+// Append.  A workgroup takes 16 token places of a sequence (one block) and one
+// key head, one value head or KV8_Q_HEADS query heads.  A code is decided next
+// to a rounding border, so keys and values are computed in 64 bits (the rate of
+// f64 is far from bounding this: the rows' bytes do), and the codes do not
+// depend on the order of any 32-bit sum.  Angles in 64 bits too, for positions
+// far out: one sine and cosine per pair and half block, the rows between by
+// rotating on.
+// ---------------------------------------------------------------------------
+struct Angle {
+  double c, s;
+};
+
+// ang[row][pair] for rows [0, nr) at positions pos0 + row.
+__device__ void block_angles(Angle* ang, uint64_t pos0, uint32_t nr, uint32_t rot, float theta) {
+  const uint32_t half = rot / 2;
+  if (half == 0) return;
+  const uint32_t teams = nr > 1 && 256u / half > 1 ? min(256u / half, nr) : 1u;
+  const uint32_t per = (nr + teams - 1) / teams;
+  for (uint32_t t = threadIdx.x; t < half * teams; t += 256) {
+    const uint32_t i = t % half, r0 = (t / half) * per, r1 = min(r0 + per, nr);
+    if (r0 >= r1) continue;
+    const double f = pow((double)theta, -2.0 * (double)i / (double)rot);
+    Angle a, st{1.0, 0.0};
+    sincos((double)(pos0 + r0) * f, &a.s, &a.c);
+    if (r1 - r0 > 1) sincos(f, &st.s, &st.c);
+    for (uint32_t r = r0; r < r1; r++) {
+      ang[r * half + i] = a;
+      a = Angle{a.c * st.c - a.s * st.s, a.c * st.s + a.s * st.c};
+    }
+  }
+}
+
+template <int NP>
+__device__ void append_q(const Kv8AppendArgs& a, const Angle* ang, uint32_t row0, uint32_t nr, uint32_t group) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t D = a.c.D, half = a.rot / 2;
+  const uint32_t h0 = group * KV8_Q_HEADS, nh = min(KV8_Q_HEADS, a.nq - h0);
+  for (uint32_t t = wave; t < nr * nh; t += 4) {
+    const uint32_t r = t / nh, h = h0 + t % nh;
+    const float* in = a.q + (uint64_t)(row0 + r) * a.qs + (uint64_t)h * D;
+    float* out = a.qo + (uint64_t)(row0 + r) * a.nq * D + (uint64_t)h * D;
+    float x0[NP], x1[NP], ss = 0.f;
+#pragma unroll
+    for (int m = 0; m < NP; m++) {
+      const uint32_t i = lane + 64 * m;
+      x0[m] = x1[m] = 0.f;
+      if (i < D / 2) {
+        uint32_t d0, d1;
+        pair_dims(i, D, a.rot, &d0, &d1);
+        x0[m] = in[d0];
+        x1[m] = in[d1];
+      }
+      ss += x0[m] * x0[m] + x1[m] * x1[m];
+    }
+    const float inv = 1.0f / sqrtf(wave_sum(ss) / (float)D + a.eps);
+#pragma unroll
+    for (int m = 0; m < NP; m++) {
+      const uint32_t i = lane + 64 * m;
+      if (i >= D / 2) continue;
+      uint32_t d0, d1;
+      pair_dims(i, D, a.rot, &d0, &d1);
+      const float u = x0[m] * inv * a.qn[d0], w = x1[m] * inv * a.qn[d1];
+      float c = 1.f, s = 0.f;
+      if (i < half) {
+        c = (float)ang[r * half + i].c;
+        s = (float)ang[r * half + i].s;
+      }
+      out[d0] = u * c - w * s;
+      out[d1] = u * s + w * c;
+    }
+  }
+}
+
+// Places of a block's element (token, dim) and 16-byte pieces.
+__device__ __forceinline__ uint32_t k_place(uint32_t t, uint32_t d) { return (d >> 4) * 256 + t * 16 + (d & 15); }
+__device__ __forceinline__ uint32_t v_place(uint32_t t, uint32_t d, uint32_t D) { return (t >> 2) * 4 * D + d * 4 + (t & 3); }
+
+template <int NP, bool IS_K>
+__device__ void append_kv(const Kv8AppendArgs& a, const Angle* ang, int8_t* tile, double* red, uint32_t row0,
+                          uint32_t o0, uint32_t nr, uint32_t head, uint64_t at) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t D = a.c.D, half = a.rot / 2, o1 = o0 + nr;
+  int8_t* codes = (IS_K ? a.c.k : a.c.v) + at * (uint64_t)(KV8_BLOCK * D);
+  float* scale = (IS_K ? a.c.ks : a.c.vs) + at;
+  const float* src = IS_K || a.k_eq_v ? a.k : a.v;
+  const float old = o0 > 0 ? *scale : 0.f;
+  // the codes already there (a fresh block's places without a token become 0)
+  int4* t4 = reinterpret_cast<int4*>(tile);
+  for (uint32_t i = threadIdx.x; i < D; i += 256) t4[i] = o0 > 0 ? reinterpret_cast<const int4*>(codes)[i] : int4{0, 0, 0, 0};
+
+  // wave w: token places 4 w .. 4 w + 3 of the block
+  double x0[4][NP], x1[4][NP], amax = 0.0;
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const uint32_t t = wave * 4 + j;
+    const bool mine = t >= o0 && t < o1;
+    const float* in = src + (uint64_t)(row0 + (mine ? t - o0 : 0)) * a.kvs + (uint64_t)head * D;
+    double ss = 0.0;
+#pragma unroll
+    for (int m = 0; m < NP; m++) {
+      const uint32_t i = lane + 64 * m;
+      x0[j][m] = x1[j][m] = 0.0;
+      if (mine && i < D / 2) {
+        uint32_t d0, d1;
+        pair_dims(i, D, a.rot, &d0, &d1);
+        x0[j][m] = (double)in[d0];
+        x1[j][m] = (double)in[d1];
+      }
+      ss += x0[j][m] * x0[j][m] + x1[j][m] * x1[j][m];
+    }
+    if (!mine) continue;
+    const double inv = 1.0 / sqrt(wave_sum(ss) / (double)D + (double)a.eps);
+#pragma unroll
+    for (int m = 0; m < NP; m++) {
+      const uint32_t i = lane + 64 * m;
+      if (i >= D / 2) continue;
+      double u = x0[j][m] * inv, w = x1[j][m] * inv;
+      if (IS_K) {
+        uint32_t d0, d1;
+        pair_dims(i, D, a.rot, &d0, &d1);
+        u *= (double)a.kn[d0];
+        w *= (double)a.kn[d1];
+        if (i < half) {
+          const Angle g = ang[(t - o0) * half + i];
+          const double y = u * g.c - w * g.s;
+          w = u * g.s + w * g.c;
+          u = y;
+        }
+      }
+      x0[j][m] = u;
+      x1[j][m] = w;
+      amax = fmax(amax, fmax(fabs(u), fabs(w)));
+      bad |= !(fabs(u) < 1e300) || !(fabs(w) < 1e300);
+    }
+  }
+  amax = wave_max(amax);
+  if (__any(bad)) amax = HUGE_VAL;
+  if (lane == 0) red[wave] = amax;
+  __syncthreads();
+  amax = fmax(fmax(red[0], red[1]), fmax(red[2], red[3]));
+
+  // least e with amax <= 127 2^e (127 = 0.9921875 * 2^7), not below f32's normal range
+  float fresh = 0.f;
+  if (amax > 0.0) {
+    int e;
+    const double m = frexp(amax, &e);
+    fresh = amax < HUGE_VAL ? (float)ldexp(1.0, max(m <= 0.9921875 ? e - 7 : e - 6, -126)) : __builtin_nanf("");
+  }
+  const float now = old != old || fresh != fresh ? __builtin_nanf("") : fmaxf(old, fresh);
+  const bool grown = o0 > 0 && now > old;
+  if (grown) {  // shift the codes already there
+    const float by = old / now;
+    for (uint32_t i = threadIdx.x; i < o0 * D; i += 256) {
+      const uint32_t t = i / D, d = i - t * D, p = IS_K ? k_place(t, d) : v_place(t, d, D);
+      tile[p] = (int8_t)(int)rintf((float)tile[p] * by);
+    }
+  }
+  const double inv = now > 0.f ? 1.0 / (double)now : 0.0;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const uint32_t t = wave * 4 + j;
+    if (t < o0 || t >= o1) continue;
+#pragma unroll
+    for (int m = 0; m < NP; m++) {
+      const uint32_t i = lane + 64 * m;
+      if (i >= D / 2) continue;
+      uint32_t d0, d1;
+      pair_dims(i, D, a.rot, &d0, &d1);
+      const int c0 = (int)rint(x0[j][m] * inv), c1 = (int)rint(x1[j][m] * inv);
+      tile[IS_K ? k_place(t, d0) : v_place(t, d0, D)] = (int8_t)min(127, max(-127, c0));
+      tile[IS_K ? k_place(t, d1) : v_place(t, d1, D)] = (int8_t)min(127, max(-127, c1));
+    }
+  }
+  __syncthreads();
+  // pieces of 16 bytes: of one token (K), of the four tokens of a group (V)
+  const uint32_t lo = grown ? 0u : o0;
+  for (uint32_t i = threadIdx.x; i < D; i += 256) {
+    const uint32_t t = IS_K ? i & 15 : (i / (D / 4)) * 4;
+    const bool out = IS_K ? t >= lo && t < o1 : t + 3 >= lo && t < o1;
+    if (out) reinterpret_cast<int4*>(codes)[i] = t4[i];
+  }
+  if (threadIdx.x == 0 && !(now == old && o0 > 0)) *scale = now;
+}
+
+// grid (2 nkv + query groups, blocks a sequence's rows can touch, sequences)
+template <int NP>
+__device__ __forceinline__ void append(const Kv8AppendArgs& a) {
+  extern __shared__ char lds[];
+  const uint32_t seq = blockIdx.z, unit = blockIdx.x;
+  uint32_t first;
+  const uint32_t rows = seq_rows(a.b, seq, &first);
+  const uint64_t past = a.b.past[seq], blk = past / KV8_BLOCK + blockIdx.y;
+  const uint64_t p0 = max(past, blk * KV8_BLOCK), p1 = min(past + rows, (blk + 1) * KV8_BLOCK);
+  if (p0 >= p1) return;
+  const uint32_t nr = (uint32_t)(p1 - p0), row0 = first + (uint32_t)(p0 - past), nkv = a.c.nkv;
+  double* red = reinterpret_cast<double*>(lds);
+  int8_t* tile = reinterpret_cast<int8_t*>(lds + 32);
+  Angle* ang = reinterpret_cast<Angle*>(lds + 32 + KV8_BLOCK * a.c.D);
+  if (unit < 2 * nkv) {
+    const uint32_t head = unit >> 1, page = page_of(a.c, a.b, seq, blk);
+    if (page >= a.c.num_pages) return;  // no page: nothing is kept
+    const uint64_t at = block_at(a.c, page, head, blk);
+    const uint32_t o0 = (uint32_t)(p0 - blk * KV8_BLOCK);
+    if (unit & 1) {
+      append_kv<NP, false>(a, ang, tile, red, row0, o0, nr, head, at);
+    } else {
+      block_angles(ang, p0, nr, a.rot, a.theta);
+      __syncthreads();
+      append_kv<NP, true>(a, ang, tile, red, row0, o0, nr, head, at);
+    }
+  } else {
+    block_angles(ang, p0, nr, a.rot, a.theta);
+    __syncthreads();
+    append_q<NP>(a, ang, row0, nr, unit - 2 * nkv);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention.  A workgroup takes 16 query columns (consecutive rows times the
+// query heads of one kv head) and a share of their tokens; its four waves take
+// the share's steps of 32 tokens in turn, each with its own running maximum
+// and sum, and are joined through LDS.
+//
+//   S^T (tokens x columns) = K . Q^T    v_mfma_i32_16x16x64_i8: the codes as they
+//       lie, Q as four signed base-256 digits of a 31-bit fixed-point number per
+//       row (the digit sums are exact; 31 bits keep what the f32 row has)
+//   O^T (dims x columns) += V^T . P^T   v_mfma_f32_16x16x32_f16: the codes as f16
+//       (exact), P times the block's scale as two f16 halves (22 bits)
+//
+// S^T leaves a lane the scores of tokens 4 g .. 4 g + 3 (g = lane / 16) of both
+// 16-token blocks of a step for its column, which is the B operand of the
+// second product: P needs no exchange between lanes.
+// P's halves hold p 2^(14 + e - E) with E the largest scale exponent so far, so
+// that they neither overflow nor lose small probabilities.
+// ---------------------------------------------------------------------------
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kNoExp = -100000;
+
+__device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
+  // byte ^ 0x80 under the exponent of 1024 is 1152 + code
+  a ^= 0x80808080u;
+  b ^= 0x80808080u;
+  union {
+    uint32_t w[4];
+    f16x2 h[4];
+    f16x8 v;
+  } u;
+  u.w[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+  u.w[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+  u.w[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+  u.w[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+  const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+#pragma unroll
+  for (int i = 0; i < 4; i++) u.h[i] = u.h[i] - off;
+  return u.v;
+}
+
+// a tile of 16 columns of one kv head of a sequence, and its token range
+struct Tile {
+  uint32_t seq, head, first, rows, col0, ncol;
+  uint64_t past, lo, hi;  // tokens [lo, hi) are visible to one of its columns
+  uint32_t step0, steps;  // steps of 32 tokens that hold them
+};
+
+// false: the tile has no row
+__device__ __forceinline__ bool tile_of(const Kv8AttnArgs& a, uint32_t seq, uint32_t head, uint32_t tile, Tile* t) {
+  const uint32_t G = a.nq / a.c.nkv;
+  t->rows = seq_rows(a.b, seq, &t->first);
+  t->seq = seq;
+  t->head = head;
+  t->col0 = tile * KV8_COLS;
+  const uint64_t cols = (uint64_t)t->rows * G;
+  if (t->col0 >= cols) return false;
+  t->ncol = (uint32_t)min((uint64_t)KV8_COLS, cols - t->col0);
+  t->past = a.b.past[seq];
+  const uint64_t p0 = t->past + t->col0 / G, p1 = t->past + (t->col0 + t->ncol - 1) / G;
+  const uint64_t lo = a.window && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
+  const uint64_t held = (uint64_t)a.b.max_pages << a.c.page_shift;  // tokens the table can name
+  const uint64_t hi = min(p1 + 1, held);
+  t->lo = lo;
+  t->hi = hi;
+  t->step0 = (uint32_t)(lo / KV8_STEP);
+  t->steps = hi > lo ? (uint32_t)((hi + KV8_STEP - 1) / KV8_STEP) - t->step0 : 0u;
+  return true;
+}
+
+template <int NL>
+struct Step {
+  i32x4 k[2][NL], v[2][NL];
+  float ks[2], vs[2];
+  bool has[2];
+};
+
+template <int NL>
+__device__ __forceinline__ void load_step(const Kv8AttnArgs& a, const Tile& t, uint32_t step, Step<NL>* s) {
+  const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, D = a.c.D;
+#pragma unroll
+  for (int b = 0; b < 2; b++) {
+    const uint64_t blk = (uint64_t)step * 2 + b;
+    const uint32_t page = page_of(a.c, a.b, t.seq, blk);
+    // a block that no column sees may hold anything, scales too
+    s->has[b] = page < a.c.num_pages && blk * KV8_BLOCK < t.hi && (blk + 1) * KV8_BLOCK > t.lo;
+    const uint64_t at = block_at(a.c, s->has[b] ? page : 0, t.head, blk);
+    s->ks[b] = a.c.ks[at];
+    s->vs[b] = a.c.vs[at];
+    const int8_t* kb = a.c.k + at * (uint64_t)(KV8_BLOCK * D);
+    const int8_t* vb = a.c.v + at * (uint64_t)(KV8_BLOCK * D);
+#pragma unroll
+    for (int l = 0; l < NL; l++) {
+      s->k[b][l] = i32x4{0, 0, 0, 0};
+      s->v[b][l] = i32x4{0, 0, 0, 0};
+      if (64 * l + 16 * g < D) s->k[b][l] = *reinterpret_cast<const i32x4*>(kb + (4 * l + g) * 256 + n * 16);
+      if (64 * l + 4 * n < D) s->v[b][l] = *reinterpret_cast<const i32x4*>(vb + g * 4 * D + (16 * l + n) * 16);
+    }
+  }
+}
+
+// A column's running softmax, and its sums in units of 2^(E - 14).
+template <int NL>
+struct Run {
+  f32x4 o[NL][4];
+  float m, l;
+  int E;
+};
+
+template <int NL>
+__device__ __forceinline__ void attend_step(const Kv8AttnArgs& a, const Step<NL>& s, const i32x4 (&qd)[4][NL],
+                                            float qmul, int64_t pos, uint32_t step, Run<NL>* r) {
+  const uint32_t g = (threadIdx.x & 63) >> 4;
+  float sc[2][4], mx = r->m;
+  int E = r->E;
+#pragma unroll
+  for (int b = 0; b < 2; b++) {
+    i32x4 acc[4];
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+      acc[d] = i32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int l = 0; l < NL; l++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.k[b][l], qd[d][l], acc[d], 0, 0, 0);
+    }
+    const float mul = qmul * s.ks[b];
+    const int64_t t0 = (int64_t)step * KV8_STEP + b * KV8_BLOCK + 4 * g;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float x = fmaf(fmaf(fmaf((float)acc[3][i], 256.f, (float)acc[2][i]), 256.f, (float)acc[1][i]), 256.f, (float)acc[0][i]);
+      const bool seen = s.has[b] && t0 + i <= pos && (a.window == 0 || t0 + i > pos - (int64_t)a.window);
+      sc[b][i] = seen ? x * mul * a.scale : -INFINITY;
+      mx = fmaxf(mx, sc[b][i]);
+    }
+    // the exponent of a scale that counts (a power of two; 0 and NaN have none)
+    if (s.has[b] && s.vs[b] > 0.f && s.vs[b] < INFINITY) E = max(E, (int)((__float_as_uint(s.vs[b]) >> 23) & 255) - 127);
+  }
+  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  const float base = mx == -INFINITY ? 0.f : mx;
+  const float alpha = exp2f((r->m - base) * kLog2e);
+  const float turn = r->E == E ? alpha : alpha * ldexpf(1.f, max(r->E - E, -200));
+  r->m = mx;
+  r->E = E;
+  union {
+    _Float16 h[8];
+    f16x8 v;
+  } hi, lo;
+  float sum = 0.f;
+#pragma unroll
+  for (int b = 0; b < 2; b++) {
+    const float vmul = ldexpf(s.vs[b], E == kNoExp ? 0 : 14 - E);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const bool seen = sc[b][i] != -INFINITY;  // (a NaN score is seen)
+      const float p = seen ? exp2f((sc[b][i] - base) * kLog2e) : 0.f;
+      sum += p;
+      const float w = seen ? p * vmul : 0.f;
+      hi.h[4 * b + i] = (_Float16)w;
+      lo.h[4 * b + i] = (_Float16)(w - (float)hi.h[4 * b + i]);
+    }
+  }
+  r->l = r->l * alpha + sum;
+  if (__any(turn != 1.f)) {
+#pragma unroll
+    for (int l = 0; l < NL; l++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) r->o[l][j] *= turn;
+  }
+#pragma unroll
+  for (int l = 0; l < NL; l++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const f16x8 v = codes_f16((uint32_t)s.v[0][l][j], (uint32_t)s.v[1][l][j]);
+      r->o[l][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi.v, r->o[l][j], 0, 0, 0);
+      r->o[l][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo.v, r->o[l][j], 0, 0, 0);
+    }
+}
+
+// The tile's query columns as digits: q = qmul_unscaled * (d3 256^3 + .. + d0).
+template <int NL>
+__device__ __forceinline__ float load_q(const Kv8AttnArgs& a, const Tile& t, i32x4 (&qd)[4][NL], int64_t* pos) {
+  const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, D = a.c.D, G = a.nq / a.c.nkv;
+  const uint32_t col = t.col0 + min(n, t.ncol - 1);  // columns past the last repeat it
+  const float* q = a.q + ((uint64_t)(t.first + col / G) * a.nq + (uint64_t)t.head * G + col % G) * D;
+  *pos = (int64_t)(t.past + col / G);
+  float amax = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int l = 0; l < NL; l++) {
+    if (64 * l + 16 * g < D) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(q + 64 * l + 16 * g + 4 * j);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          amax = fmaxf(amax, fabsf(x[i]));
+          bad |= !(fabsf(x[i]) < INFINITY);
+        }
+      }
+    }
+  }
+  amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+  amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+  int any = bad ? 1 : 0;
+  any |= __shfl_xor(any, 16, 64);
+  any |= __shfl_xor(any, 32, 64);
+  int e = 0;
+  if (!any) frexpf(amax, &e);
+#pragma unroll
+  for (int l = 0; l < NL; l++) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      if (!any && 64 * l + 16 * g < D) x = *reinterpret_cast<const f32x4*>(q + 64 * l + 16 * g + 4 * j);
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        int v = (int)rintf(ldexpf(x[i], 30 - e));
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+          const int digit = (int)(int8_t)(v & 255);
+          w[d] |= (uint32_t)(digit & 255) << (8 * i);
+          v = (v - digit) >> 8;
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < 4; d++) qd[d][l][j] = (int)w[d];
+    }
+  }
+  return any ? __builtin_nanf("") : ldexpf(1.f, e - 30);
+}
+
+// grid (tiles * splits, kv heads, sequences)
+template <int NL>
+__device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
+  extern __shared__ char lds[];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const uint32_t D = a.c.D, G = a.nq / a.c.nkv;
+  const uint32_t split = blockIdx.x % a.nsplit, tile = blockIdx.x / a.nsplit;
+  Tile t;
+  if (!tile_of(a, blockIdx.z, blockIdx.y, tile, &t)) return;
+  const uint32_t per = kv8_split_steps(t.steps, a.nsplit, a.chunk);
+  const uint32_t s0 = t.step0 + split * per, end = t.step0 + t.steps;
+  if (split > 0 && s0 >= end) return;
+  const uint32_t s1 = min(s0 + per, end);
+
+  i32x4 qd[4][NL];
+  int64_t pos;
+  const float qmul = load_q<NL>(a, t, qd, &pos);
+  Run<NL> r;
+#pragma unroll
+  for (int l = 0; l < NL; l++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) r.o[l][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  r.m = -INFINITY;
+  r.l = 0.f;
+  r.E = kNoExp;
+  for (uint32_t s = s0 + wave; s < s1; s += 4) {
+    Step<NL> st;
+    load_step<NL>(a, t, s, &st);
+    attend_step<NL>(a, st, qd, qmul, pos, s, &r);
+  }
+  r.l += __shfl_xor(r.l, 16, 64);
+  r.l += __shfl_xor(r.l, 32, 64);
+
+  // join the waves: m and l of all, then o by a tree through LDS
+  float* lm = reinterpret_cast<float*>(lds);  // [4][16]
+  float* ll = lm + 64;
+  float* lo = ll + 64;  // [2 waves][16 NL floats][64 lanes]
+  if (lane < 16) {
+    lm[wave * 16 + n] = r.m;
+    ll[wave * 16 + n] = r.l;
+  }
+  __syncthreads();
+  float M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; w++) M = fmaxf(M, lm[w * 16 + n]);
+  const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+  for (int w = 0; w < 4; w++) L += ll[w * 16 + n] * exp2f((lm[w * 16 + n] - base) * kLog2e);
+  const float f = exp2f((r.m - base) * kLog2e), fe = r.E == kNoExp ? 0.f : ldexpf(f, r.E - 14);
+#pragma unroll
+  for (int l = 0; l < NL; l++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) r.o[l][j] *= fe;
+#pragma unroll
+  for (int half = 2; half >= 1; half >>= 1) {
+    if (wave >= half && wave < 2 * half) {
+      float* to = lo + (wave - half) * (16 * NL * 64);
+#pragma unroll
+      for (int l = 0; l < NL; l++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) to[(l * 16 + j * 4 + i) * 64 + lane] = r.o[l][j][i];
+    }
+    __syncthreads();
+    if (wave < half) {
+      const float* from = lo + wave * (16 * NL * 64);
+#pragma unroll
+      for (int l = 0; l < NL; l++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) r.o[l][j][i] += from[(l * 16 + j * 4 + i) * 64 + lane];
+    }
+    __syncthreads();
+  }
+  if (wave != 0 || n >= t.ncol) return;
+  const bool whole = per >= t.steps;  // the only split that runs
+  const uint32_t col = t.col0 + n;
+  float* to;
+  float by = 1.f;
+  if (whole) {
+    to = a.out + ((uint64_t)(t.first + col / G) * a.nq + (uint64_t)t.head * G + col % G) * D;
+    by = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;  // nothing visible: 0
+  } else {
+    const uint64_t unit = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / a.nsplit) + tile;
+    to = a.part + ((unit * a.nsplit + split) * KV8_COLS + n) * (D + 2);
+    if (g == 0) {
+      to[D] = M;
+      to[D + 1] = L;
+    }
+  }
+#pragma unroll
+  for (int l = 0; l < NL; l++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t d = 64 * l + 16 * g + 4 * i;
+      if (d < D) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) to[d + j] = r.o[l][j][i] * by;
+      }
+    }
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_append_p1_k(Kv8AppendArgs a) { append<1>(a); }
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_append_p2_k(Kv8AppendArgs a) { append<2>(a); }
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_append_p4_k(Kv8AppendArgs a) { append<4>(a); }
+
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_attn_l1_k(Kv8AttnArgs a) { attend<1>(a); }
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_attn_l2_k(Kv8AttnArgs a) { attend<2>(a); }
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_attn_l4_k(Kv8AttnArgs a) { attend<4>(a); }
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_attn_l8_k(Kv8AttnArgs a) { attend<8>(a); }
+
+// Joins the splits of a tile, in split order.  grid (tiles * 16 columns, kv heads,
+// sequences), a workgroup a column.
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a) {
+  const uint32_t tile = blockIdx.x / KV8_COLS, n = blockIdx.x % KV8_COLS, D = a.c.D, G = a.nq / a.c.nkv;
+  Tile t;
+  if (!tile_of(a, blockIdx.z, blockIdx.y, tile, &t) || n >= t.ncol) return;
+  const uint32_t per = kv8_split_steps(t.steps, a.nsplit, a.chunk);
+  if (per >= t.steps) return;  // written by its only split
+  const uint32_t live = (t.steps + per - 1) / per;
+  const uint64_t unit = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / KV8_COLS) + tile;
+  const uint64_t row = KV8_COLS * (uint64_t)(D + 2);
+  const float* p = a.part + unit * a.nsplit * row + n * (uint64_t)(D + 2);
+  float M = -INFINITY, L = 0.f;
+  for (uint32_t s = 0; s < live; s++) M = fmaxf(M, p[s * row + D]);
+  const float base = M == -INFINITY ? 0.f : M;
+  for (uint32_t s = 0; s < live; s++) L += p[s * row + D + 1] * exp2f((p[s * row + D] - base) * kLog2e);
+  const float by = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;
+  const uint32_t col = t.col0 + n;
+  float* out = a.out + ((uint64_t)(t.first + col / G) * a.nq + (uint64_t)t.head * G + col % G) * D;
+  for (uint32_t d = threadIdx.x; d < D; d += 256) {
+    float o = 0.f;
+    for (uint32_t s = 0; s < live; s++) o += p[s * row + d] * exp2f((p[s * row + D] - base) * kLog2e);
+    out[d] = o * by;
+  }
+}
+
+// Read-back: the rows that a batch names as the values their codes stand for;
+// rows of places without a page are 0.  grid (kv heads, blocks, sequences)
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_read_k(Kv8ReadArgs a) {
+  const uint32_t seq = blockIdx.z, head = blockIdx.x, D = a.c.D;
+  uint32_t first;
+  const uint32_t rows = seq_rows(a.b, seq, &first);
+  const uint64_t past = a.b.past[seq], blk = past / KV8_BLOCK + blockIdx.y;
+  const uint64_t p0 = max(past, blk * KV8_BLOCK), p1 = min(past + rows, (blk + 1) * KV8_BLOCK);
+  if (p0 >= p1) return;
+  const uint32_t o0 = (uint32_t)(p0 - blk * KV8_BLOCK), o1 = (uint32_t)(p1 - blk * KV8_BLOCK);
+  const uint64_t row0 = first + (p0 - past), kv = (uint64_t)a.c.nkv * D;
+  const uint32_t page = page_of(a.c, a.b, seq, blk);
+  const bool has = page < a.c.num_pages;
+  const uint64_t at = block_at(a.c, has ? page : 0, head, blk);
+  union Piece {
+    int4 w;
+    int8_t b[16];
+  };
+  for (uint32_t i = threadIdx.x; i < 2 * D; i += 256) {
+    const bool is_k = i < D;
+    float* out = is_k ? a.k : a.v;
+    if (!out) continue;
+    const uint32_t j = is_k ? i : i - D;
+    Piece p;
+    p.w = int4{0, 0, 0, 0};
+    if (has) p.w = reinterpret_cast<const int4*>((is_k ? a.c.k : a.c.v) + at * (uint64_t)(KV8_BLOCK * D))[j];
+    const float s = has ? (is_k ? a.c.ks : a.c.vs)[at] : 0.f;
+    if (is_k) {
+      const uint32_t t = j & 15, d = (j >> 4) * 16;
+      if (t < o0 || t >= o1) continue;
+      float* to = out + (row0 + t - o0) * kv + (uint64_t)head * D + d;
+#pragma unroll
+      for (int e = 0; e < 16; e++) to[e] = (float)p.b[e] * s;
+    } else {
+      const uint32_t grp = j / (D / 4), d = (j % (D / 4)) * 4;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const uint32_t t = grp * 4 + e;
+        if (t < o0 || t >= o1) continue;
+        float* to = out + (row0 + t - o0) * kv + (uint64_t)head * D + d;
+#pragma unroll
+        for (int r = 0; r < 4; r++) to[r] = (float)p.b[4 * r + e] * s;
+      }
+    }
+  }
+}

@@ -43,7 +43,8 @@ static std::string library_dir() {
 
 // Code objects built by ai-research_amd/build.py next to libgemma_hip.so.
 static const char* kCodeObjects[] = {"gh_gemv.hsaco", "gh_gemv_norm.hsaco", "gh_util.hsaco",
-                                     "gh_attn.hsaco", "gh_norm.hsaco", "gh_prefill.hsaco"};
+                                     "gh_attn.hsaco", "gh_norm.hsaco", "gh_prefill.hsaco",
+                                     "gh_kv8.hsaco", "gh_sample.hsaco"};
 
 }  // namespace gh
 

@@ -1,0 +1,314 @@
+// serving.cpp -- entry points of batched serving: the paged 8-bit K/V cache
+// (append, read-back, attention), probabilities from logits, and the verification
+// of drafted tokens.  Argument checks, launch shapes, and the launch on the
+// context stream.  Nothing here allocates: a caller gives the workspace.
+#include <math.h>
+
+#include <new>
+#include <string>
+
+#include "../common/kv8_args.h"
+#include "../common/sample_args.h"
+#include "runtime.hpp"
+
+using gh::fail;
+
+namespace {
+
+// No exception leaves a C entry.
+template <typename F>
+gh_status guarded(const char* who, F f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return fail(GH_ERR_ALLOC, "out of host memory");
+  } catch (...) {
+    return fail(GH_ERR_INVALID, who);
+  }
+}
+
+gh_status invalid(const char* who, const char* what) { return fail(GH_ERR_INVALID, std::string(who) + ": " + what); }
+gh_status unsupported(const char* who, const char* what) {
+  return fail(GH_ERR_UNSUPPORTED, std::string(who) + ": " + what);
+}
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// The first launch of a kernel asks the code objects for it in turn; the answer
+// "not found" of one stays behind as HIP's last error, which a host's other HIP
+// code in this thread would take for its own.
+gh_status launch(gh_context* ctx, const char* name, dim3 grid, dim3 block, unsigned lds, void** args) {
+  const hipFunction_t f = ctx->fn(name);
+  if (hipPeekAtLastError() == hipErrorNotFound) (void)hipGetLastError();
+  if (!f) return fail(GH_ERR_CODE_OBJECT, std::string("kernel not found in the code objects: ") + name);
+  return ctx->launch(name, grid, block, lds, args);
+}
+
+constexpr uint32_t kMaxRows = 1000000u, kMaxGrid = 65535u;
+
+gh_status check_cache(const char* who, const gh_kv8_cache* c, Kv8View* v) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return invalid(who, "cache is null or has a null pointer");
+  if (c->num_pages == 0 || c->num_kv == 0 || c->head_dim == 0) return invalid(who, "cache has a zero size");
+  if (c->num_pages == 0xffffffffu) return unsupported(who, "num_pages must be below 2^32 - 1");
+  if (c->page_tokens < KV8_BLOCK || c->page_tokens > 256 || (c->page_tokens & (c->page_tokens - 1)))
+    return unsupported(who, "page_tokens must be 16, 32, 64, 128 or 256");
+  if (c->head_dim % 16 || c->head_dim > 512) return unsupported(who, "head_dim must be a multiple of 16 up to 512");
+  if (c->num_kv > 4096) return unsupported(who, "more than 4096 kv heads");
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
+    return invalid(who, "cache codes must be 16-byte aligned, scales 4-byte");
+  uint32_t shift = 4;
+  while ((1u << shift) < c->page_tokens) shift++;
+  *v = Kv8View{static_cast<int8_t*>(c->k), static_cast<int8_t*>(c->v), c->k_scale, c->v_scale, c->num_pages, shift,
+               c->num_kv, c->head_dim};
+  return GH_OK;
+}
+
+gh_status check_batch(const char* who, const gh_kv8_batch* b, Kv8Rows* r) {
+  if (!b) return invalid(who, "batch is null");
+  *r = Kv8Rows{b->seq_start, b->past, b->pages, b->num_seqs, b->max_pages, b->num_rows, b->max_rows};
+  if (b->num_seqs == 0 || b->num_rows == 0 || b->max_rows == 0) return GH_OK;  // nothing to do
+  if (!b->seq_start || !b->past || !b->pages) return invalid(who, "batch has a null pointer");
+  if (b->max_pages == 0) return invalid(who, "max_pages is zero");
+  if (!aligned(b->seq_start, 4) || !aligned(b->past, 4) || !aligned(b->pages, 4))
+    return invalid(who, "batch arrays must be 4-byte aligned");
+  if (b->num_seqs > kMaxGrid) return unsupported(who, "more than 65535 sequences");
+  if (b->num_rows > kMaxRows) return unsupported(who, "more than 1000000 rows");
+  r->max_rows = std::min(b->max_rows, b->num_rows);
+  return GH_OK;
+}
+
+bool empty(const Kv8Rows& r) { return r.num_seqs == 0 || r.num_rows == 0 || r.max_rows == 0; }
+
+// Blocks that a sequence's rows can touch.
+uint32_t touched(const Kv8Rows& r) { return (r.max_rows + KV8_BLOCK - 2) / KV8_BLOCK + 1; }
+
+struct AttnPlan {
+  uint32_t tiles = 0, nsplit = 1, chunk = 4;
+  size_t bytes = 0;
+};
+
+// Splits of the token range: enough workgroups for two a CU.  A split takes at
+// least a step for each of its four waves.
+gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, const Kv8Rows& r, uint32_t num_q,
+                    uint32_t window, uint32_t max_kv, AttnPlan* p) {
+  if (num_q == 0 || num_q % c.nkv) return invalid(who, "num_q must be a positive multiple of the kv heads");
+  if (num_q > 65536) return unsupported(who, "more than 65536 query heads");
+  *p = AttnPlan{};
+  if (empty(r)) return GH_OK;
+  const uint64_t G = num_q / c.nkv, tiles = (r.max_rows * G + KV8_COLS - 1) / KV8_COLS;
+  uint64_t tokens = (uint64_t)r.max_pages << c.page_shift;
+  if (max_kv) tokens = std::min<uint64_t>(tokens, max_kv);
+  if (window) tokens = std::min<uint64_t>(tokens, (uint64_t)window + (KV8_COLS + G - 1) / G);
+  const uint64_t steps = tokens / KV8_STEP + 1, units = tiles * c.nkv * r.num_seqs;
+  const uint64_t most = std::min<uint64_t>((steps + p->chunk - 1) / p->chunk, KV8_MAX_SPLIT);
+  const uint64_t want = (2ull * ctx->num_cus + units - 1) / units;
+  p->nsplit = (uint32_t)std::max<uint64_t>(1, std::min(want, most));
+  if (tiles * p->nsplit > 0x7fffffffull) return unsupported(who, "too many query rows");
+  p->tiles = (uint32_t)tiles;
+  if (p->nsplit > 1) p->bytes = (size_t)units * p->nsplit * KV8_COLS * (c.D + 2) * sizeof(float);
+  return GH_OK;
+}
+
+uint32_t chunks_of(uint32_t vocab) { return (uint32_t)(((uint64_t)vocab + SAMPLE_CHUNK - 1) / SAMPLE_CHUNK); }
+
+gh_status check_work(const char* who, const void* work, size_t have, size_t need) {
+  if (need == 0) return GH_OK;
+  if (!work || have < need) return invalid(who, "workspace is null or smaller than the workspace function says");
+  if (!aligned(work, 16)) return invalid(who, "workspace must be 16-byte aligned");
+  return GH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t gh_kv8_code_bytes(const gh_kv8_cache* c) {
+  return c ? (size_t)c->num_pages * c->page_tokens * c->num_kv * c->head_dim : 0;
+}
+size_t gh_kv8_scale_bytes(const gh_kv8_cache* c) {
+  return c ? (size_t)c->num_pages * (c->page_tokens / KV8_BLOCK) * c->num_kv * sizeof(float) : 0;
+}
+
+gh_status gh_kv8_append(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8_batch* batch, const float* Q_in,
+                        const float* K_in, const float* V_in, uint32_t q_stride, uint32_t kv_stride,
+                        const float* Q_norm, const float* K_norm, float* Q_out, uint32_t num_q, uint32_t rotary_dim,
+                        uint32_t k_eq_v, float theta, float eps) {
+  return guarded("gh_kv8_append", [&]() -> gh_status {
+    const char* who = "gh_kv8_append";
+    if (!ctx) return invalid(who, "ctx is null");
+    Kv8AppendArgs a{};
+    gh_status st = check_cache(who, cache, &a.c);
+    if (st != GH_OK) return st;
+    if ((st = check_batch(who, batch, &a.b)) != GH_OK) return st;
+    if (rotary_dim > a.c.D || rotary_dim % 2) return invalid(who, "rotary_dim must be even and at most head_dim");
+    if (!(theta > 0.f) || !(theta < INFINITY)) return invalid(who, "theta must be positive");
+    if (!(eps >= 0.f) || !(eps < INFINITY)) return invalid(who, "eps must not be negative");
+    if (num_q > 65536) return unsupported(who, "more than 65536 query heads");
+    if (empty(a.b)) return GH_OK;
+    if (!K_in || !K_norm || (!V_in && !k_eq_v)) return invalid(who, "K_in, V_in or K_norm is null");
+    if (num_q && (!Q_in || !Q_norm || !Q_out)) return invalid(who, "Q_in, Q_norm or Q_out is null");
+    if (kv_stride < (uint64_t)a.c.nkv * a.c.D || (num_q && q_stride < (uint64_t)num_q * a.c.D))
+      return invalid(who, "a row stride is shorter than its heads");
+    for (const void* p : {(const void*)Q_in, (const void*)K_in, (const void*)V_in, (const void*)Q_norm,
+                          (const void*)K_norm, (const void*)Q_out})
+      if (!aligned(p, 4)) return invalid(who, "rows and norms must be 4-byte aligned");
+    a.q = Q_in;
+    a.k = K_in;
+    a.v = V_in ? V_in : K_in;
+    a.qn = Q_norm;
+    a.kn = K_norm;
+    a.qo = Q_out;
+    a.qs = q_stride;
+    a.kvs = kv_stride;
+    a.nq = num_q;
+    a.rot = rotary_dim;
+    a.k_eq_v = k_eq_v ? 1 : 0;
+    a.theta = theta;
+    a.eps = eps;
+    const uint32_t rows = std::min(a.b.max_rows, KV8_BLOCK);
+    const unsigned lds = 32 + KV8_BLOCK * a.c.D + rows * (rotary_dim / 2) * 16;
+    const dim3 grid(2 * a.c.nkv + (num_q + KV8_Q_HEADS - 1) / KV8_Q_HEADS, touched(a.b), a.b.num_seqs);
+    const char* name = a.c.D <= 128 ? "gh_kv8_append_p1_k" : a.c.D <= 256 ? "gh_kv8_append_p2_k" : "gh_kv8_append_p4_k";
+    void* args[] = {&a};
+    return launch(ctx, name, grid, dim3(256), lds, args);
+  });
+}
+
+gh_status gh_kv8_read(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8_batch* batch, float* K_out,
+                      float* V_out) {
+  return guarded("gh_kv8_read", [&]() -> gh_status {
+    const char* who = "gh_kv8_read";
+    if (!ctx) return invalid(who, "ctx is null");
+    Kv8ReadArgs a{};
+    gh_status st = check_cache(who, cache, &a.c);
+    if (st != GH_OK) return st;
+    if ((st = check_batch(who, batch, &a.b)) != GH_OK) return st;
+    if (!K_out && !V_out) return invalid(who, "K_out and V_out are null");
+    if (!aligned(K_out, 4) || !aligned(V_out, 4)) return invalid(who, "rows must be 4-byte aligned");
+    if (empty(a.b)) return GH_OK;
+    a.k = K_out;
+    a.v = V_out;
+    void* args[] = {&a};
+    return launch(ctx, "gh_kv8_read_k", dim3(a.c.nkv, touched(a.b), a.b.num_seqs), dim3(256), 0, args);
+  });
+}
+
+size_t gh_kv8_attn_workspace(const gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8_batch* batch,
+                             uint32_t num_q, uint32_t window, uint32_t max_kv) {
+  size_t bytes = 0;
+  guarded("gh_kv8_attn_workspace", [&]() -> gh_status {
+    const char* who = "gh_kv8_attn_workspace";
+    if (!ctx) return invalid(who, "ctx is null");
+    Kv8View c;
+    Kv8Rows r;
+    AttnPlan p;
+    gh_status st = check_cache(who, cache, &c);
+    if (st == GH_OK) st = check_batch(who, batch, &r);
+    if (st == GH_OK) st = plan_attn(who, ctx, c, r, num_q, window, max_kv, &p);
+    bytes = p.bytes;
+    return st;
+  });
+  return bytes;
+}
+
+gh_status gh_kv8_attn(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8_batch* batch, const float* Q,
+                      float* out, uint32_t num_q, float scale, uint32_t window, uint32_t max_kv, void* work,
+                      size_t work_bytes) {
+  return guarded("gh_kv8_attn", [&]() -> gh_status {
+    const char* who = "gh_kv8_attn";
+    if (!ctx) return invalid(who, "ctx is null");
+    Kv8AttnArgs a{};
+    AttnPlan p;
+    gh_status st = check_cache(who, cache, &a.c);
+    if (st != GH_OK) return st;
+    if ((st = check_batch(who, batch, &a.b)) != GH_OK) return st;
+    if ((st = plan_attn(who, ctx, a.c, a.b, num_q, window, max_kv, &p)) != GH_OK) return st;
+    if (!(fabsf(scale) < INFINITY)) return invalid(who, "scale must be finite");
+    if (empty(a.b)) return GH_OK;
+    if (!Q || !out) return invalid(who, "Q or out is null");
+    if (!aligned(Q, 16) || !aligned(out, 16)) return invalid(who, "Q and out must be 16-byte aligned");
+    if ((st = check_work(who, work, work_bytes, p.bytes)) != GH_OK) return st;
+    a.q = Q;
+    a.out = out;
+    a.part = static_cast<float*>(work);
+    a.nq = num_q;
+    a.window = window;
+    a.nsplit = p.nsplit;
+    a.chunk = p.chunk;
+    a.scale = scale;
+    const uint32_t nl = a.c.D <= 64 ? 1 : a.c.D <= 128 ? 2 : a.c.D <= 256 ? 4 : 8;
+    const char* name = nl == 1   ? "gh_kv8_attn_l1_k"
+                       : nl == 2 ? "gh_kv8_attn_l2_k"
+                       : nl == 4 ? "gh_kv8_attn_l4_k"
+                                 : "gh_kv8_attn_l8_k";
+    void* args[] = {&a};
+    st = launch(ctx, name, dim3(p.tiles * p.nsplit, a.c.nkv, a.b.num_seqs), dim3(256), 512 + 8192 * nl, args);
+    if (st != GH_OK || p.nsplit == 1) return st;
+    return launch(ctx, "gh_kv8_merge_k", dim3(p.tiles * KV8_COLS, a.c.nkv, a.b.num_seqs), dim3(256), 0, args);
+  });
+}
+
+size_t gh_logit_probs_workspace(const gh_context*, uint32_t rows, uint32_t vocab) {
+  return (size_t)rows * chunks_of(vocab) * 2 * sizeof(float);
+}
+
+gh_status gh_logit_probs(gh_context* ctx, const float* logits, float* probs, uint32_t rows, uint32_t vocab,
+                         uint32_t stride, float softcap, float temperature, void* work, size_t work_bytes) {
+  return guarded("gh_logit_probs", [&]() -> gh_status {
+    const char* who = "gh_logit_probs";
+    if (!ctx) return invalid(who, "ctx is null");
+    if (stride < vocab) return invalid(who, "stride is shorter than a row");
+    if (!(softcap >= 0.f) || !(softcap < INFINITY)) return invalid(who, "softcap must be 0 (none) or positive");
+    if (!(temperature > 0.f) || !(temperature < INFINITY)) return invalid(who, "temperature must be positive");
+    if (rows > kMaxGrid) return unsupported(who, "more than 65535 rows");
+    if (rows == 0 || vocab == 0) return GH_OK;
+    if (!logits || !probs) return invalid(who, "logits or probs is null");
+    if (!aligned(logits, 4) || !aligned(probs, 4)) return invalid(who, "rows must be 4-byte aligned");
+    gh_status st = check_work(who, work, work_bytes, gh_logit_probs_workspace(ctx, rows, vocab));
+    if (st != GH_OK) return st;
+    ProbsArgs a{logits, probs, static_cast<float*>(work), stride, vocab, chunks_of(vocab), softcap,
+                (float)(1.4426950408889634 / (double)temperature)};
+    if (!(a.mul < INFINITY)) return invalid(who, "temperature is too small");
+    const bool vec = vocab % 4 == 0 && stride % 4 == 0 && aligned(logits, 16) && aligned(probs, 16);
+    void* args[] = {&a};
+    const dim3 grid(a.chunks, rows);
+    st = launch(ctx, vec ? "gh_probs_part_v4_k" : "gh_probs_part_v1_k", grid, dim3(256), 0, args);
+    if (st != GH_OK) return st;
+    return launch(ctx, vec ? "gh_probs_write_v4_k" : "gh_probs_write_v1_k", grid, dim3(256), 0, args);
+  });
+}
+
+size_t gh_spec_verify_workspace(const gh_context*, uint32_t num_seqs, uint32_t vocab) {
+  return (size_t)num_seqs * chunks_of(vocab) * 2 * sizeof(double);
+}
+
+gh_status gh_spec_verify(gh_context* ctx, const float* target, const float* draft, const uint32_t* tokens,
+                         const uint32_t* n_draft, const float* u, const float* pick, uint32_t* out_tokens,
+                         uint32_t* accepted, uint32_t num_seqs, uint32_t max_draft, uint32_t vocab, void* work,
+                         size_t work_bytes) {
+  return guarded("gh_spec_verify", [&]() -> gh_status {
+    const char* who = "gh_spec_verify";
+    if (!ctx) return invalid(who, "ctx is null");
+    if (num_seqs > kMaxGrid) return unsupported(who, "more than 65535 sequences");
+    if (max_draft > 65535) return unsupported(who, "more than 65535 drafted tokens");
+    if (vocab == 0) return invalid(who, "vocab is zero");
+    if (vocab > 0x7fffffffu) return unsupported(who, "vocab must be below 2^31");
+    if (num_seqs == 0) return GH_OK;
+    if (!target || !pick || !out_tokens || !accepted || (max_draft && (!tokens || !u)))
+      return invalid(who, "null pointer");
+    for (const void* p : {(const void*)target, (const void*)draft, (const void*)tokens, (const void*)n_draft,
+                          (const void*)u, (const void*)pick, (const void*)out_tokens, (const void*)accepted})
+      if (!aligned(p, 4)) return invalid(who, "arrays must be 4-byte aligned");
+    gh_status st = check_work(who, work, work_bytes, gh_spec_verify_workspace(ctx, num_seqs, vocab));
+    if (st != GH_OK) return st;
+    VerifyArgs a{target, draft, tokens, n_draft, u, pick, out_tokens, accepted, static_cast<double*>(work),
+                 max_draft, vocab, chunks_of(vocab)};
+    const bool vec = vocab % 4 == 0 && aligned(target, 16) && aligned(draft, 16);
+    void* args[] = {&a};
+    st = launch(ctx, vec ? "gh_verify_part_v4_k" : "gh_verify_part_v1_k", dim3(a.chunks, num_seqs), dim3(256), 0, args);
+    if (st != GH_OK) return st;
+    return launch(ctx, "gh_verify_token_k", dim3(num_seqs), dim3(256), 0, args);
+  });
+}
+
+}  // extern "C"

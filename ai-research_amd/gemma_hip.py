@@ -89,6 +89,37 @@ _SIGS.update({
     "gh_norm_gemv_argmax_bf16": (_i, [_vp, _vp, _vp, _vp, _u32, _u32, C.POINTER(XPrologue)]),
 })
 
+class Kv8Cache(C.Structure):
+    """gh_kv8_cache: the paged 8-bit K/V cache (device addresses and sizes)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("num_pages", _u32),
+                ("page_tokens", _u32), ("num_kv", _u32), ("head_dim", _u32)]
+
+
+class Kv8Batch(C.Structure):
+    """gh_kv8_batch: the ragged rows of a call (device addresses and bounds)."""
+    _fields_ = [("seq_start", _vp), ("past", _vp), ("pages", _vp), ("num_seqs", _u32),
+                ("max_pages", _u32), ("num_rows", _u32), ("max_rows", _u32)]
+
+
+_pc, _pb = C.POINTER(Kv8Cache), C.POINTER(Kv8Batch)
+_SIGS.update({
+    "gh_kv8_code_bytes": (_sz, [_pc]),
+    "gh_kv8_scale_bytes": (_sz, [_pc]),
+    "gh_kv8_append": (_i, [_vp, _pc, _pb] + [_vp] * 3 + [_u32] * 2 + [_vp] * 3 + [_u32] * 3 +
+                      [_f32, _f32]),
+    "gh_kv8_read": (_i, [_vp, _pc, _pb, _vp, _vp]),
+    "gh_kv8_attn_workspace": (_sz, [_vp, _pc, _pb, _u32, _u32, _u32]),
+    "gh_kv8_attn": (_i, [_vp, _pc, _pb, _vp, _vp, _u32, _f32, _u32, _u32, _vp, _sz]),
+    "gh_logit_probs_workspace": (_sz, [_vp, _u32, _u32]),
+    "gh_logit_probs": (_i, [_vp, _vp, _vp, _u32, _u32, _u32, _f32, _f32, _vp, _sz]),
+    "gh_spec_verify_workspace": (_sz, [_vp, _u32, _u32]),
+    "gh_spec_verify": (_i, [_vp] * 9 + [_u32] * 3 + [_vp, _sz]),
+})
+
+NO_TOKEN = 0xffffffff  # GH_NO_TOKEN
+KV8_BLOCK = 16         # GH_KV8_BLOCK
+
+
 class ModelConfig(C.Structure):
     """gh_model_config (ModelConfig, src/model/types.zig:43-61)."""
     _fields_ = [("vocab_size", _u32), ("hidden_size", _u32), ("intermediate_size", _u32),
@@ -423,11 +454,54 @@ class Context:
         _check(lib().gh_prefill_gate_up_geglu(self.h, mode, _addr(Wg), _addr(Wu), _addr(A),
                                               _addr(act), T, N, K), "gh_prefill_gate_up_geglu")
 
+    # ---- batched serving: paged 8-bit K/V cache, probabilities, drafted tokens
+    def kv8_append(self, cache, batch, Q_in, K_in, V_in, q_stride, kv_stride, Q_norm, K_norm, Q_out,
+                   num_q, rotary_dim, k_eq_v, theta, eps=1e-6):
+        _check(lib().gh_kv8_append(self.h, C.byref(cache), C.byref(batch), _opt(Q_in), _addr(K_in),
+                                   _opt(V_in), q_stride, kv_stride, _opt(Q_norm), _addr(K_norm),
+                                   _opt(Q_out), num_q, rotary_dim, int(k_eq_v), theta, eps),
+               "gh_kv8_append")
+
+    def kv8_read(self, cache, batch, K_out, V_out):
+        _check(lib().gh_kv8_read(self.h, C.byref(cache), C.byref(batch), _opt(K_out), _opt(V_out)),
+               "gh_kv8_read")
+
+    def kv8_attn_workspace(self, cache, batch, num_q, window=0, max_kv=0):
+        return lib().gh_kv8_attn_workspace(self.h, C.byref(cache), C.byref(batch), num_q, window,
+                                           max_kv)
+
+    def kv8_attn(self, cache, batch, Q, out, num_q, scale=1.0, window=0, max_kv=0, work=None,
+                 work_bytes=0):
+        _check(lib().gh_kv8_attn(self.h, C.byref(cache), C.byref(batch), _addr(Q), _addr(out), num_q,
+                                 scale, window, max_kv, _opt(work), work_bytes), "gh_kv8_attn")
+
+    def logit_probs_workspace(self, rows, vocab):
+        return lib().gh_logit_probs_workspace(self.h, rows, vocab)
+
+    def logit_probs(self, logits, probs, rows, vocab, stride, softcap, temperature, work, work_bytes):
+        _check(lib().gh_logit_probs(self.h, _addr(logits), _addr(probs), rows, vocab, stride, softcap,
+                                    temperature, _opt(work), work_bytes), "gh_logit_probs")
+
+    def spec_verify_workspace(self, num_seqs, vocab):
+        return lib().gh_spec_verify_workspace(self.h, num_seqs, vocab)
+
+    def spec_verify(self, target, draft, tokens, n_draft, u, pick, out_tokens, accepted, num_seqs,
+                    max_draft, vocab, work, work_bytes):
+        _check(lib().gh_spec_verify(self.h, _addr(target), _opt(draft), _opt(tokens), _opt(n_draft),
+                                    _opt(u), _addr(pick), _addr(out_tokens), _addr(accepted),
+                                    num_seqs, max_draft, vocab, _opt(work), work_bytes),
+               "gh_spec_verify")
+
 
 def _addr(b):
     if isinstance(b, Buffer):
         return b.ptr
     return int(b)
+
+
+def _opt(b):
+    """The address of an argument that may be absent."""
+    return None if b is None else _addr(b)
 
 
 class Ring:

@@ -285,6 +285,117 @@ gh_status gh_prefill_gate_up_geglu(gh_context *ctx, gh_quant_mode mode, const vo
                                    const void *Wu, const float *A, float *act, uint32_t T,
                                    uint32_t N, uint32_t K);
 
+/* ---- batched serving: the paged 8-bit K/V cache, sampling probabilities and
+ * drafted tokens (no reference counterpart: the reference serves one sequence
+ * over an f32 ring and samples greedily).  All array arguments are device
+ * pointers; nothing here allocates, so every call may be captured; a call
+ * whose workspace function gives more than 0 bytes needs that many (16-byte
+ * aligned, not shared with a call that may run at the same time), and the
+ * same sizes in the same arguments give the same answer.
+ *
+ * A page holds page_tokens tokens of every kv head, in blocks of
+ * GH_KV8_BLOCK tokens.  A block of one kv head has one scale for its keys and
+ * one for its values, a power of two: an element is code * scale, code in
+ * -127 .. 127.  Layout, pages one after another:
+ *   k       int8 [num_pages][num_kv][blocks][head_dim / 16][16 tokens][16 dims]
+ *   v       int8 [num_pages][num_kv][blocks][4][head_dim][4 tokens]
+ *   *_scale f32  [num_pages][num_kv][blocks]
+ * with blocks = page_tokens / 16; v's element (token 4 a + b, dim d) of a block
+ * lies at [a][d][b].  page_tokens is 16, 32, 64, 128 or 256; head_dim a
+ * multiple of 16 up to 512; k and v 16-byte aligned.  Fresh memory needs no
+ * clearing. */
+#define GH_KV8_BLOCK 16
+typedef struct gh_kv8_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  uint32_t num_pages, page_tokens, num_kv, head_dim;
+} gh_kv8_cache;
+/* Bytes of k (and of v), and of k_scale (and of v_scale). */
+size_t gh_kv8_code_bytes(const gh_kv8_cache *cache);
+size_t gh_kv8_scale_bytes(const gh_kv8_cache *cache);
+
+/* The rows of a call, ragged: sequence s has rows seq_start[s] ..
+ * seq_start[s + 1] - 1 (none when they are equal), which are its tokens past[s],
+ * past[s] + 1, ...; token t lies in page pages[s * max_pages + t / page_tokens].
+ * The host gives bounds: num_rows for the rows in all (entries above it count as
+ * it), max_rows for those of one sequence (further ones are not handled).  A
+ * token past the table's end, or whose entry is not below num_pages, has no
+ * page: it is not kept, reads as 0 and is attended to by no one.  Sequences may
+ * share pages that are read; a page that a call appends to must be named once.
+ * Rows of arguments that belong to no sequence are not touched. */
+typedef struct gh_kv8_batch {
+  const uint32_t *seq_start, *past, *pages;
+  uint32_t num_seqs, max_pages, num_rows, max_rows;
+} gh_kv8_batch;
+
+/* gh_qkv_rope for a batch, into the paged cache: per row, RMSNorm(q_norm) +
+ * split-half RoPE on the first rotary_dim dims of every query head into Q_out
+ * [num_rows][num_q * head_dim]; RMSNorm(k_norm) + RoPE of each key head and
+ * unit-RMS of each value head (the raw key head when k_eq_v) into the cache at
+ * the row's token.  Q_in has rows q_stride floats apart, K_in and V_in kv_stride
+ * (they may lie in one packed [q|k|v] row); Q_out may be Q_in when q_stride is
+ * num_q * head_dim.  num_q 0 appends only.  Angles, keys and values are computed
+ * in 64 bits up to the code (half to even).
+ *
+ * A block's scale is the least power of two whose 127-fold reaches the largest
+ * magnitude written to the block since its first token was last written (at
+ * least 2^-126; 0 for a block of zeros).  Appending a larger one raises the
+ * scale and rounds the codes before it again: an element is off by at most half
+ * a step of the scale it was written at, plus half a step for each rise since,
+ * under one step in all.  Appending at a block's first token starts the block
+ * anew, so a sequence may be cut back (past lowered) and written again.  A row
+ * with a NaN or infinite element makes the scales of its block NaN until then. */
+gh_status gh_kv8_append(gh_context *ctx, const gh_kv8_cache *cache, const gh_kv8_batch *batch,
+                        const float *Q_in, const float *K_in, const float *V_in,
+                        uint32_t q_stride, uint32_t kv_stride, const float *Q_norm,
+                        const float *K_norm, float *Q_out, uint32_t num_q, uint32_t rotary_dim,
+                        uint32_t k_eq_v, float theta, float eps);
+/* The values that the cache holds for the batch's rows: K_out and V_out
+ * [num_rows][num_kv * head_dim], either may be null. */
+gh_status gh_kv8_read(gh_context *ctx, const gh_kv8_cache *cache, const gh_kv8_batch *batch,
+                      float *K_out, float *V_out);
+/* gh_decode_attn for a batch over the paged cache: out row = softmax over the
+ * tokens t of its sequence with t <= its own and, when window > 0, t > its own -
+ * window, of scale * (Q . K[t]), times V[t]; query head h reads kv head h /
+ * (num_q / num_kv).  Q and out are [num_rows][num_q * head_dim], 16-byte
+ * aligned.  A row that sees no token is 0.  The rows' own tokens must be in the
+ * cache (gh_kv8_append).  max_kv: about the most tokens of a sequence, its rows
+ * included (0: what the table holds); it and the window set how the work is
+ * split, not what is computed. */
+size_t gh_kv8_attn_workspace(const gh_context *ctx, const gh_kv8_cache *cache,
+                             const gh_kv8_batch *batch, uint32_t num_q, uint32_t window,
+                             uint32_t max_kv);
+gh_status gh_kv8_attn(gh_context *ctx, const gh_kv8_cache *cache, const gh_kv8_batch *batch,
+                      const float *Q, float *out, uint32_t num_q, float scale, uint32_t window,
+                      uint32_t max_kv, void *work, size_t work_bytes);
+/* probs = softmax(y / temperature) of each row, y = softcap * tanh(logit /
+ * softcap), or the logit when softcap is 0; a logit of -inf is masked (0) either
+ * way, and a row of them gives zeros; a row with a NaN (or, without a softcap, a
+ * +inf) gives NaN.  Rows are stride floats apart in both; probs may be logits. */
+size_t gh_logit_probs_workspace(const gh_context *ctx, uint32_t rows, uint32_t vocab);
+gh_status gh_logit_probs(gh_context *ctx, const float *logits, float *probs, uint32_t rows,
+                         uint32_t vocab, uint32_t stride, float softcap, float temperature,
+                         void *work, size_t work_bytes);
+/* Speculative sampling.  Sequence s has n = n_draft[s] drafted tokens (at most
+ * max_draft; n_draft null: max_draft each) tokens[s][max_draft], drawn from
+ * draft [num_seqs][max_draft][vocab] (null: certain, q = 1), and the target's
+ * probabilities target [num_seqs][max_draft + 1][vocab].  In order, draft i is
+ * kept while u[s][i] * q_i(x_i) < p_i(x_i); a token that is no vocab index is not.
+ * One more token is drawn with pick[s] in [0, 1): the least v with cumsum(w)[v] >
+ * pick * sum(w), where w = max(p_i - q_i, 0) at the first draft i not kept (p_i
+ * when that is all zero), or p_n after the last; NaN and negative weights count
+ * as 0.  out_tokens [num_seqs][max_draft + 1] gets the kept drafts, the drawn
+ * token and GH_NO_TOKEN after it; accepted[s] the number kept.  Where no weight
+ * is positive, or their sum is infinite, the drawn token is GH_NO_TOKEN.  Sums
+ * are in 64 bits. */
+#define GH_NO_TOKEN 0xffffffffu
+size_t gh_spec_verify_workspace(const gh_context *ctx, uint32_t num_seqs, uint32_t vocab);
+gh_status gh_spec_verify(gh_context *ctx, const float *target, const float *draft,
+                         const uint32_t *tokens, const uint32_t *n_draft, const float *u,
+                         const float *pick, uint32_t *out_tokens, uint32_t *accepted,
+                         uint32_t num_seqs, uint32_t max_draft, uint32_t vocab, void *work,
+                         size_t work_bytes);
+
 /* ---- ring bookkeeping: DynamicRingBuffer (src/ring_buffer.zig:7-147) -------
  * The host side of the [anchors | window | recall] ring: which slot a clock
  * maps to and which slots a token attends over.  The K/V values live in the

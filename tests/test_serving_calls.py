@@ -1,0 +1,101 @@
+"""The batched serving calls' checks of their arguments and what they launch, on a HIP
+runtime without a device (tests/host_checks)."""
+import os
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+INVALID, UNSUPPORTED = 4, 5
+
+
+@pytest.fixture(scope="module")
+def serving(tmp_path_factory):
+    out = tmp_path_factory.mktemp("serving")
+    here, runtime = os.path.join(ROOT, "tests", "host_checks"), os.path.join(ROOT, "ai-research_amd", "csrc", "runtime")
+    sources = [os.path.join(runtime, s + ".cpp") for s in ("runtime", "engine", "model", "ring", "serving")]
+    sources += [os.path.join(here, s) for s in ("fake_hip.cpp", "fake_errors.cpp", "serving.cpp")]
+    exe = str(out / "serving")
+    objs = [str(out / ("%d.o" % i)) for i in range(len(sources))]
+    jobs = [subprocess.Popen(["g++", "-O1", "-std=c++17", "-pthread", "-D__HIP_PLATFORM_AMD__", "-w",
+                              "-I", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"),
+                              "-I", os.path.join(ROOT, "include"), "-I", os.path.dirname(runtime), "-I", here,
+                              "-c", s, "-o", o]) for s, o in zip(sources, objs)]
+    assert all(j.wait() == 0 for j in jobs)
+    subprocess.run(["g++", "-pthread", *objs, "-ldl", "-o", exe], check=True)
+    (out / "gh_gemv.hsaco").write_bytes(b"")
+
+    def ask(call, *changes):
+        r = subprocess.run([exe, str(out), call], input="".join("%s %s\n" % c for c in changes), capture_output=True, text=True,
+                           timeout=60)
+        assert r.returncode == 0, r.stderr
+        got = []
+        for line in r.stdout.splitlines():
+            st, need, why, kernels = line.split("\t")
+            got.append((int(st), int(need), why, [tuple(k.split()) for k in kernels.split(";") if k]))
+        assert len(got) == len(changes)
+        return got
+
+    return ask
+
+
+CACHE = [("ctx", 0, INVALID), ("cache", 0, INVALID), ("batch", 0, INVALID), ("k", 0, INVALID), ("v_scale", 0, INVALID),
+         ("k", 4104, INVALID), ("num_pages", 0, INVALID), ("num_pages", 4294967295, UNSUPPORTED), ("page_tokens", 8, UNSUPPORTED),
+         ("page_tokens", 48, UNSUPPORTED), ("page_tokens", 512, UNSUPPORTED), ("head_dim", 0, INVALID), ("head_dim", 72, UNSUPPORTED),
+         ("head_dim", 528, UNSUPPORTED), ("num_kv", 0, INVALID), ("seq_start", 0, INVALID), ("pages", 0, INVALID),
+         ("past", 4098, INVALID), ("max_pages", 0, INVALID), ("num_seqs", 65536, UNSUPPORTED), ("num_rows", 1000001, UNSUPPORTED)]
+REFUSED = {
+    "append": CACHE + [("q", 0, INVALID), ("kin", 0, INVALID), ("vin", 0, INVALID), ("kn", 0, INVALID), ("out", 0, INVALID),
+                       ("q_stride", 255, INVALID), ("kv_stride", 127, INVALID), ("rot", 66, INVALID), ("rot", 3, INVALID),
+                       ("theta", 0, INVALID), ("theta", "nan", INVALID), ("theta", "inf", INVALID), ("eps", -1, INVALID),
+                       ("eps", "nan", INVALID), ("num_q", 65537, UNSUPPORTED), ("kin", 4097, INVALID)],
+    "read": CACHE + [("kin", 4097, INVALID)],
+    "attn": CACHE + [("q", 0, INVALID), ("out", 0, INVALID), ("q", 4100, INVALID), ("num_q", 0, INVALID), ("num_q", 5, INVALID),
+                     ("num_q", 65538, UNSUPPORTED), ("scale", "nan", INVALID), ("scale", "inf", INVALID), ("work", 0, INVALID), ("work", 4104, INVALID),
+                     ("bytes", 1, INVALID)],
+    "probs": [("ctx", 0, INVALID), ("q", 0, INVALID), ("out", 0, INVALID), ("out", 4097, INVALID), ("stride", 999, INVALID),
+              ("cap", -1, INVALID), ("cap", "nan", INVALID), ("temp", 0, INVALID), ("temp", -1, INVALID), ("temp", "nan", INVALID),
+              ("temp", 1e-39, INVALID), ("rows", 65536, UNSUPPORTED), ("work", 0, INVALID), ("bytes", 1, INVALID)],
+    "verify": [("ctx", 0, INVALID), ("q", 0, INVALID), ("tokens", 0, INVALID), ("u", 0, INVALID), ("pick", 0, INVALID), ("out", 0, INVALID),
+               ("accepted", 0, INVALID), ("vocab", 0, INVALID), ("vocab", 2147483648, UNSUPPORTED), ("num_seqs", 65536, UNSUPPORTED),
+               ("max_draft", 65536, UNSUPPORTED), ("draft", 4097, INVALID), ("work", 0, INVALID), ("bytes", 1, INVALID)],
+}
+
+
+@pytest.mark.parametrize("call", sorted(REFUSED))
+def test_refusals_have_a_status_and_a_message_and_launch_nothing(serving, call):
+    cases = REFUSED[call]
+    for (name, value, want), (st, _, why, kernels) in zip(cases, serving(call, *[c[:2] for c in cases])):
+        assert st == want and not kernels, (name, value, st, why)
+        assert why.startswith("gh_"), (name, value, why)
+
+
+@pytest.mark.parametrize("call,names", [("append", ("num_seqs", "num_rows", "max_rows")), ("read", ("num_seqs", "num_rows")),
+                                        ("attn", ("num_seqs", "num_rows", "max_rows")), ("probs", ("rows", "vocab")),
+                                        ("verify", ("num_seqs",))])
+def test_nothing_to_do_is_no_error(serving, call, names):
+    for st, need, why, kernels in serving(call, *[(n, 0) for n in names]):
+        assert (st, need, kernels) == (0, 0, []), why
+
+
+def test_arguments_that_may_be_absent(serving):
+    assert serving("append", ("k_eq_v", 1))[0][0] == 0
+    assert serving("append", ("num_q", 0))[0][0] == 0
+    for name in ("kin", "vin"):
+        assert serving("read", (name, 0))[0][0] == 0
+    for name in ("draft", "n_draft", "max_draft"):
+        assert serving("verify", (name, 0))[0][0] == 0
+
+
+def test_grids_cover_the_rows(serving):
+    # a sequence's rows can begin at a block's last token: 9 rows touch 2 blocks, 18 rows 3
+    for rows, blocks in ((1, 1), (2, 2), (9, 2), (17, 2), (18, 3)):
+        (_, _, _, kernels), = serving("append", ("max_rows", rows))
+        name, x, y, z, block, lds = kernels[0]
+        assert (x, y, z) == (str(2 * 2 + 1), str(blocks), "3")
+        assert int(lds) == 32 + 16 * 64 + min(rows, 16) * 32 * 16
+    # 4 query heads over 2 kv heads: 2 columns a row, 16 a tile
+    for rows, tiles in ((1, 1), (8, 1), (9, 2)):
+        (_, need, _, kernels), = serving("attn", ("max_rows", rows))
+        assert [int(k) for k in kernels[0][1:4]][1:] == [2, 3] and int(kernels[0][1]) % tiles == 0
+        assert (need > 0) == (len(kernels) == 2)
