@@ -26,8 +26,10 @@ DEVICE_FLAGS = ["--offload-arch=gfx950", "--genco", "--no-gpu-bundle-output", "-
 KERNEL_FAMILIES = ["gemv", "gemv_norm", "util", "attn", "norm", "prefill", "kv8", "sample"]
 
 # Per-family extra flags.  The prefill GEMMs scale each 32-block's MFMA sum on
-# the VALU; in VGPR form the MFMA results need no v_accvgpr_read first.
-FAMILY_FLAGS = {"prefill": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# the VALU, the attention rescales its sums there; in VGPR form the MFMA results
+# need no v_accvgpr_read first.
+FAMILY_FLAGS = {"prefill": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                "kv8": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 HOST_SOURCES = ["runtime.cpp", "engine.cpp", "model.cpp", "ring.cpp", "serving.cpp"]
 HIP_HOST_SOURCES = ["noalloc.hip"]

@@ -335,6 +335,7 @@ __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
 struct Tile {
   uint32_t seq, head, first, rows, col0, ncol;
   uint64_t past, lo, hi;  // tokens [lo, hi) are visible to one of its columns
+  uint64_t all_lo, all_hi; // tokens [all_lo, all_hi) to every one of them, where there is a page
   uint32_t step0, steps;  // steps of 32 tokens that hold them
 };
 
@@ -355,38 +356,47 @@ __device__ __forceinline__ bool tile_of(const Kv8AttnArgs& a, uint32_t seq, uint
   const uint64_t hi = min(p1 + 1, held);
   t->lo = lo;
   t->hi = hi;
+  t->all_lo = a.window && p1 + 1 > a.window ? p1 + 1 - a.window : 0;
+  t->all_hi = p0 + 1;
   t->step0 = (uint32_t)(lo / KV8_STEP);
   t->steps = hi > lo ? (uint32_t)((hi + KV8_STEP - 1) / KV8_STEP) - t->step0 : 0u;
   return true;
 }
 
+// A step's codes of keys or values in registers, with its scales.
 template <int NL>
-struct Step {
-  i32x4 k[2][NL], v[2][NL];
-  float ks[2], vs[2];
+struct Codes {
+  i32x4 c[2][NL];
+  float s[2];
   bool has[2];
 };
 
-template <int NL>
-__device__ __forceinline__ void load_step(const Kv8AttnArgs& a, const Tile& t, uint32_t step, Step<NL>* s) {
+// The pages of 32 of a wave's steps (s, s + 4, ...), two blocks each, in its lanes.
+__device__ __forceinline__ uint32_t step_pages(const Kv8AttnArgs& a, const Tile& t, uint32_t s) {
+  const uint32_t lane = threadIdx.x & 63;
+  const uint64_t blk = 2 * ((uint64_t)s + 4 * (lane >> 1)) + (lane & 1);
+  // a block that no column sees may hold anything, scales too
+  const bool some = blk * KV8_BLOCK < t.hi && (blk + 1) * KV8_BLOCK > t.lo;
+  return some ? page_of(a.c, a.b, t.seq, blk) : a.c.num_pages;
+}
+
+template <int NL, bool IS_K>
+__device__ __forceinline__ void load_codes(const Kv8AttnArgs& a, const Tile& t, uint32_t step, uint32_t pages, uint32_t i,
+                                           Codes<NL>* s) {
   const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, D = a.c.D;
 #pragma unroll
   for (int b = 0; b < 2; b++) {
     const uint64_t blk = (uint64_t)step * 2 + b;
-    const uint32_t page = page_of(a.c, a.b, t.seq, blk);
-    // a block that no column sees may hold anything, scales too
-    s->has[b] = page < a.c.num_pages && blk * KV8_BLOCK < t.hi && (blk + 1) * KV8_BLOCK > t.lo;
+    const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)(2 * i + b));
+    s->has[b] = page < a.c.num_pages;
     const uint64_t at = block_at(a.c, s->has[b] ? page : 0, t.head, blk);
-    s->ks[b] = a.c.ks[at];
-    s->vs[b] = a.c.vs[at];
-    const int8_t* kb = a.c.k + at * (uint64_t)(KV8_BLOCK * D);
-    const int8_t* vb = a.c.v + at * (uint64_t)(KV8_BLOCK * D);
+    s->s[b] = (IS_K ? a.c.ks : a.c.vs)[at];
+    const int8_t* c = (IS_K ? a.c.k : a.c.v) + at * (uint64_t)(KV8_BLOCK * D);
 #pragma unroll
     for (int l = 0; l < NL; l++) {
-      s->k[b][l] = i32x4{0, 0, 0, 0};
-      s->v[b][l] = i32x4{0, 0, 0, 0};
-      if (64 * l + 16 * g < D) s->k[b][l] = *reinterpret_cast<const i32x4*>(kb + (4 * l + g) * 256 + n * 16);
-      if (64 * l + 4 * n < D) s->v[b][l] = *reinterpret_cast<const i32x4*>(vb + g * 4 * D + (16 * l + n) * 16);
+      s->c[b][l] = i32x4{0, 0, 0, 0};
+      const uint32_t place = IS_K ? (4 * l + g) * 256 + n * 16 : g * 4 * D + (16 * l + n) * 16;
+      if ((IS_K ? 64 * l + 16 * g : 64 * l + 4 * n) < D) s->c[b][l] = *reinterpret_cast<const i32x4*>(c + place);
     }
   }
 }
@@ -400,36 +410,40 @@ struct Run {
 };
 
 template <int NL>
-__device__ __forceinline__ void attend_step(const Kv8AttnArgs& a, const Step<NL>& s, const i32x4 (&qd)[4][NL],
-                                            float qmul, int64_t pos, uint32_t step, Run<NL>* r) {
-  const uint32_t g = (threadIdx.x & 63) >> 4;
-  float sc[2][4], mx = r->m;
+__device__ __forceinline__ void clear(Run<NL>* r) {
+#pragma unroll
+  for (int l = 0; l < NL; l++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) r->o[l][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  r->m = -INFINITY;
+  r->l = 0.f;
+  r->E = kNoExp;
+}
+
+// The four digit sums of a score.  Two at a time are exact as integers (at most
+// 257 * 128 * 127 * 512 < 2^31).
+__device__ __forceinline__ float digit_sum(int d3, int d2, int d1, int d0) {
+  return fmaf((float)((d3 << 8) + d2), 65536.f, (float)((d1 << 8) + d0));
+}
+
+// The softmax of a step's scores sc (-inf: not seen): the halves of P for the
+// second product, and the running values.
+template <int NL>
+__device__ __forceinline__ void soft_step(const float (&sc)[2][4], const float (&vs)[2], const bool (&has)[2], Run<NL>* r,
+                                          f16x8* phi, f16x8* plo) {
+  float mx = r->m;
   int E = r->E;
 #pragma unroll
   for (int b = 0; b < 2; b++) {
-    i32x4 acc[4];
 #pragma unroll
-    for (int d = 0; d < 4; d++) {
-      acc[d] = i32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int l = 0; l < NL; l++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.k[b][l], qd[d][l], acc[d], 0, 0, 0);
-    }
-    const float mul = qmul * s.ks[b];
-    const int64_t t0 = (int64_t)step * KV8_STEP + b * KV8_BLOCK + 4 * g;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float x = fmaf(fmaf(fmaf((float)acc[3][i], 256.f, (float)acc[2][i]), 256.f, (float)acc[1][i]), 256.f, (float)acc[0][i]);
-      const bool seen = s.has[b] && t0 + i <= pos && (a.window == 0 || t0 + i > pos - (int64_t)a.window);
-      sc[b][i] = seen ? x * mul * a.scale : -INFINITY;
-      mx = fmaxf(mx, sc[b][i]);
-    }
+    for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[b][i]);
     // the exponent of a scale that counts (a power of two; 0 and NaN have none)
-    if (s.has[b] && s.vs[b] > 0.f && s.vs[b] < INFINITY) E = max(E, (int)((__float_as_uint(s.vs[b]) >> 23) & 255) - 127);
+    if (has[b] && vs[b] > 0.f && vs[b] < INFINITY) E = max(E, (int)((__float_as_uint(vs[b]) >> 23) & 255) - 127);
   }
   mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
   mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
   const float base = mx == -INFINITY ? 0.f : mx;
-  const float alpha = exp2f((r->m - base) * kLog2e);
+  const float alpha = __builtin_amdgcn_exp2f((r->m - base) * kLog2e);
   const float turn = r->E == E ? alpha : alpha * ldexpf(1.f, max(r->E - E, -200));
   r->m = mx;
   r->E = E;
@@ -440,11 +454,11 @@ __device__ __forceinline__ void attend_step(const Kv8AttnArgs& a, const Step<NL>
   float sum = 0.f;
 #pragma unroll
   for (int b = 0; b < 2; b++) {
-    const float vmul = ldexpf(s.vs[b], E == kNoExp ? 0 : 14 - E);
+    const float vmul = ldexpf(vs[b], E == kNoExp ? 0 : 14 - E);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const bool seen = sc[b][i] != -INFINITY;  // (a NaN score is seen)
-      const float p = seen ? exp2f((sc[b][i] - base) * kLog2e) : 0.f;
+      const float p = __builtin_amdgcn_exp2f((sc[b][i] - base) * kLog2e);
       sum += p;
       const float w = seen ? p * vmul : 0.f;
       hi.h[4 * b + i] = (_Float16)w;
@@ -458,74 +472,148 @@ __device__ __forceinline__ void attend_step(const Kv8AttnArgs& a, const Step<NL>
 #pragma unroll
       for (int j = 0; j < 4; j++) r->o[l][j] *= turn;
   }
+  *phi = hi.v;
+  *plo = lo.v;
+}
+
+// Whether the column at token pos sees token t.
+__device__ __forceinline__ bool visible(int64_t t, int64_t pos, uint32_t window) {
+  return t <= pos && (window == 0 || t > pos - (int64_t)window);
+}
+
+// Scores of a step's tokens 4 g .. of both blocks for a lane's column; -inf: not seen.
+template <int NL>
+__device__ __forceinline__ void score_step(const Kv8AttnArgs& a, const Codes<NL>& k, const i32x4* qd, float qmul,
+                                           const Tile& t, int64_t pos, uint32_t step, float (&sc)[2][4]) {
+  const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
+  i32x4 acc[2][4];
+  asm volatile("" ::: "memory");  // the digits are read in every step, not held
+#pragma unroll
+  for (int d = 0; d < 4; d++) acc[0][d] = acc[1][d] = i32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int l = 0; l < NL; l++) {
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+      const i32x4 q = qd[(d * NL + l) * 64 + lane];
+      acc[0][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k.c[0][l], q, acc[0][d], 0, 0, 0);
+      acc[1][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k.c[1][l], q, acc[1][d], 0, 0, 0);
+    }
+  }
+  // every token of the step is seen by every column
+  const bool whole = k.has[0] && k.has[1] && (uint64_t)step * KV8_STEP >= t.all_lo && ((uint64_t)step + 1) * KV8_STEP <= t.all_hi;
+#pragma unroll
+  for (int b = 0; b < 2; b++) {
+    const float mul = qmul * k.s[b];
+#pragma unroll
+    for (int i = 0; i < 4; i++) sc[b][i] = digit_sum(acc[b][3][i], acc[b][2][i], acc[b][1][i], acc[b][0][i]) * mul * a.scale;
+    if (!whole) {
+      const int64_t t0 = (int64_t)step * KV8_STEP + b * KV8_BLOCK + 4 * g;
+#pragma unroll
+      for (int i = 0; i < 4; i++) sc[b][i] = k.has[b] && visible(t0 + i, pos, a.window) ? sc[b][i] : -INFINITY;
+    }
+  }
+}
+
+template <int NL>
+__device__ __forceinline__ void value_step(const Codes<NL>& v, f16x8 hi, f16x8 lo, Run<NL>* r) {
 #pragma unroll
   for (int l = 0; l < NL; l++)
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const f16x8 v = codes_f16((uint32_t)s.v[0][l][j], (uint32_t)s.v[1][l][j]);
-      r->o[l][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi.v, r->o[l][j], 0, 0, 0);
-      r->o[l][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo.v, r->o[l][j], 0, 0, 0);
+      const f16x8 x = codes_f16((uint32_t)v.c[0][l][j], (uint32_t)v.c[1][l][j]);
+      r->o[l][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, r->o[l][j], 0, 0, 0);
+      r->o[l][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, r->o[l][j], 0, 0, 0);
     }
 }
 
-// The tile's query columns as digits: q = qmul_unscaled * (d3 256^3 + .. + d0).
+// The address of a column's row of one head.
+__device__ __forceinline__ uint64_t row_at(const Kv8AttnArgs& a, const Tile& t, uint32_t col) {
+  const uint32_t G = a.nq / a.c.nkv;
+  return ((uint64_t)(t.first + col / G) * a.nq + (uint64_t)t.head * G + col % G) * a.c.D;
+}
+
+// Signed base-256 digits of four 31-bit numbers, digit by digit: digit d of v is
+// byte d of (v + 0x80808080) ^ 0x80808080.
+__device__ __forceinline__ void digits4(const int (&v)[4], int (&w)[4]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) u[i] = ((uint32_t)v[i] + 0x80808080u) ^ 0x80808080u;
+  // bytes of u[0], u[1] in turn, then of all four
+  const uint32_t a0 = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), a1 = __builtin_amdgcn_perm(u[1], u[0], 0x07030602u);
+  const uint32_t b0 = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u), b1 = __builtin_amdgcn_perm(u[3], u[2], 0x07030602u);
+  w[0] = (int)__builtin_amdgcn_perm(b0, a0, 0x05040100u);
+  w[1] = (int)__builtin_amdgcn_perm(b0, a0, 0x07060302u);
+  w[2] = (int)__builtin_amdgcn_perm(b1, a1, 0x05040100u);
+  w[3] = (int)__builtin_amdgcn_perm(b1, a1, 0x07060302u);
+}
+
+// The tile's query columns as digits in LDS, qd[digit][l][lane] (dims 64 l + 16 g
+// .. of column n); a wave makes every fourth l.  A row's largest magnitude (joined
+// through qm) decides its unit, which is returned (NaN where the row has a NaN or
+// an infinity).
 template <int NL>
-__device__ __forceinline__ float load_q(const Kv8AttnArgs& a, const Tile& t, i32x4 (&qd)[4][NL], int64_t* pos) {
-  const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, D = a.c.D, G = a.nq / a.c.nkv;
-  const uint32_t col = t.col0 + min(n, t.ncol - 1);  // columns past the last repeat it
-  const float* q = a.q + ((uint64_t)(t.first + col / G) * a.nq + (uint64_t)t.head * G + col % G) * D;
-  *pos = (int64_t)(t.past + col / G);
+__device__ __forceinline__ float stage_q(const Kv8AttnArgs& a, const float* q, float* qm, i32x4* qd) {
+  constexpr int NS = (NL + 3) / 4;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4, D = a.c.D;
+  f32x4 x[NS][4];
   float amax = 0.f;
   bool bad = false;
 #pragma unroll
-  for (int l = 0; l < NL; l++) {
-    if (64 * l + 16 * g < D) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(q + 64 * l + 16 * g + 4 * j);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          amax = fmaxf(amax, fabsf(x[i]));
-          bad |= !(fabsf(x[i]) < INFINITY);
-        }
-      }
-    }
-  }
-  amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-  amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-  int any = bad ? 1 : 0;
-  any |= __shfl_xor(any, 16, 64);
-  any |= __shfl_xor(any, 32, 64);
-  int e = 0;
-  if (!any) frexpf(amax, &e);
-#pragma unroll
-  for (int l = 0; l < NL; l++) {
+  for (int i = 0; i < NS; i++)
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-      if (!any && 64 * l + 16 * g < D) x = *reinterpret_cast<const f32x4*>(q + 64 * l + 16 * g + 4 * j);
-      uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        int v = (int)rintf(ldexpf(x[i], 30 - e));
-#pragma unroll
-        for (int d = 0; d < 4; d++) {
-          const int digit = (int)(int8_t)(v & 255);
-          w[d] |= (uint32_t)(digit & 255) << (8 * i);
-          v = (v - digit) >> 8;
-        }
-      }
-#pragma unroll
-      for (int d = 0; d < 4; d++) qd[d][l][j] = (int)w[d];
+      const uint32_t d = 64 * (wave + 4 * i) + 16 * g + 4 * j;
+      x[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (d < D) x[i][j] = *reinterpret_cast<const f32x4*>(q + d);
     }
+#pragma unroll
+  for (int i = 0; i < NS; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        amax = fmaxf(amax, fabsf(x[i][j][c]));
+        bad |= !(fabsf(x[i][j][c]) < INFINITY);
+      }
+  if (bad) amax = INFINITY;
+  amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+  amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+  if (lane < 16) qm[wave * 16 + n] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; w++) amax = fmaxf(amax, qm[w * 16 + n]);
+  bad = amax == INFINITY;
+  int e = 0;
+  if (!bad) frexpf(amax, &e);
+#pragma unroll
+  for (int i = 0; i < NS; i++) {
+    const uint32_t l = wave + 4 * i;
+    if (l >= NL) continue;
+    i32x4 w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      int v[4], u[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++) v[c] = bad ? 0 : (int)rintf(ldexpf(x[i][j][c], 30 - e));
+      digits4(v, u);
+#pragma unroll
+      for (int d = 0; d < 4; d++) w[d][j] = u[d];
+    }
+#pragma unroll
+    for (int d = 0; d < 4; d++) qd[(d * NL + l) * 64 + lane] = w[d];
   }
-  return any ? __builtin_nanf("") : ldexpf(1.f, e - 30);
+  __syncthreads();
+  return bad ? __builtin_nanf("") : ldexpf(1.f, e - 30);
 }
 
+// Few query columns (one tile): the workgroup's waves take its steps in turn.  The
+// tokens' bytes bound it, so a wave has the next step's keys on the way while it
+// weighs this step's values, and the next values while it scores; the query
+// digits are in LDS to leave the registers to them.
 // grid (tiles * splits, kv heads, sequences)
 template <int NL>
 __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
-  extern __shared__ char lds[];
+  extern __shared__ __align__(16) char lds[];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
   const uint32_t D = a.c.D, G = a.nq / a.c.nkv;
   const uint32_t split = blockIdx.x % a.nsplit, tile = blockIdx.x / a.nsplit;
@@ -536,29 +624,42 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   if (split > 0 && s0 >= end) return;
   const uint32_t s1 = min(s0 + per, end);
 
-  i32x4 qd[4][NL];
-  int64_t pos;
-  const float qmul = load_q<NL>(a, t, qd, &pos);
+  float* lm = reinterpret_cast<float*>(lds);         // [4][16]
+  float* ll = lm + 64;                               // [4][16]
+  i32x4* qd = reinterpret_cast<i32x4*>(lds + 512);   // [4][NL][64]
+  float* lo = reinterpret_cast<float*>(lds + 512);   // [2 waves][16 NL floats][64 lanes], after the steps
+  uint32_t pages = step_pages(a, t, s0 + wave);
+  const uint32_t col = t.col0 + min(n, t.ncol - 1);  // columns past the last repeat it
+  const int64_t pos = (int64_t)(t.past + col / G);
+  Codes<NL> k, v;
+  uint32_t i = 0, s = s0 + wave;
+  if (s < s1) {
+    load_codes<NL, true>(a, t, s, pages, 0, &k);
+    load_codes<NL, false>(a, t, s, pages, 0, &v);
+  }
+  const float qmul = stage_q<NL>(a, a.q + row_at(a, t, col), lm, qd);
   Run<NL> r;
-#pragma unroll
-  for (int l = 0; l < NL; l++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) r.o[l][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  r.m = -INFINITY;
-  r.l = 0.f;
-  r.E = kNoExp;
-  for (uint32_t s = s0 + wave; s < s1; s += 4) {
-    Step<NL> st;
-    load_step<NL>(a, t, s, &st);
-    attend_step<NL>(a, st, qd, qmul, pos, s, &r);
+  clear<NL>(&r);
+  for (; s < s1; s += 4) {
+    float sc[2][4];
+    score_step<NL>(a, k, qd, qmul, t, pos, s, sc);
+    const bool more = s + 4 < s1;
+    if (++i == 32 && more) {
+      i = 0;
+      pages = step_pages(a, t, s + 4);
+    }
+    if (more) load_codes<NL, true>(a, t, s + 4, pages, i, &k);
+    __builtin_amdgcn_sched_barrier(0);
+    f16x8 hi, lo;
+    soft_step<NL>(sc, v.s, v.has, &r, &hi, &lo);
+    value_step<NL>(v, hi, lo, &r);
+    if (more) load_codes<NL, false>(a, t, s + 4, pages, i, &v);
+    __builtin_amdgcn_sched_barrier(0);
   }
   r.l += __shfl_xor(r.l, 16, 64);
   r.l += __shfl_xor(r.l, 32, 64);
 
   // join the waves: m and l of all, then o by a tree through LDS
-  float* lm = reinterpret_cast<float*>(lds);  // [4][16]
-  float* ll = lm + 64;
-  float* lo = ll + 64;  // [2 waves][16 NL floats][64 lanes]
   if (lane < 16) {
     lm[wave * 16 + n] = r.m;
     ll[wave * 16 + n] = r.l;
@@ -569,8 +670,8 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   for (int w = 0; w < 4; w++) M = fmaxf(M, lm[w * 16 + n]);
   const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
-  for (int w = 0; w < 4; w++) L += ll[w * 16 + n] * exp2f((lm[w * 16 + n] - base) * kLog2e);
-  const float f = exp2f((r.m - base) * kLog2e), fe = r.E == kNoExp ? 0.f : ldexpf(f, r.E - 14);
+  for (int w = 0; w < 4; w++) L += ll[w * 16 + n] * __builtin_amdgcn_exp2f((lm[w * 16 + n] - base) * kLog2e);
+  const float f = __builtin_amdgcn_exp2f((r.m - base) * kLog2e), fe = r.E == kNoExp ? 0.f : ldexpf(f, r.E - 14);
 #pragma unroll
   for (int l = 0; l < NL; l++)
 #pragma unroll
@@ -599,16 +700,15 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
     __syncthreads();
   }
   if (wave != 0 || n >= t.ncol) return;
-  const bool whole = per >= t.steps;  // the only split that runs
-  const uint32_t col = t.col0 + n;
+  const bool only = per >= t.steps;  // the only split that runs
   float* to;
   float by = 1.f;
-  if (whole) {
-    to = a.out + ((uint64_t)(t.first + col / G) * a.nq + (uint64_t)t.head * G + col % G) * D;
+  if (only) {
+    to = a.out + row_at(a, t, col);
     by = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;  // nothing visible: 0
   } else {
     const uint64_t unit = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / a.nsplit) + tile;
-    to = a.part + ((unit * a.nsplit + split) * KV8_COLS + n) * (D + 2);
+    to = a.part + ((unit * a.nsplit + split) * KV8_COLS + n) * (D + KV8_PART);
     if (g == 0) {
       to[D] = M;
       to[D + 1] = L;
@@ -619,10 +719,7 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const uint32_t d = 64 * l + 16 * g + 4 * i;
-      if (d < D) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) to[d + j] = r.o[l][j][i] * by;
-      }
+      if (d < D) *reinterpret_cast<f32x4*>(to + d) = f32x4{r.o[l][0][i], r.o[l][1][i], r.o[l][2][i], r.o[l][3][i]} * by;
     }
 }
 
@@ -632,33 +729,54 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_append_p1_k(Kv8AppendAr
 extern "C" __global__ __launch_bounds__(256) void gh_kv8_append_p2_k(Kv8AppendArgs a) { append<2>(a); }
 extern "C" __global__ __launch_bounds__(256) void gh_kv8_append_p4_k(Kv8AppendArgs a) { append<4>(a); }
 
-extern "C" __global__ __launch_bounds__(256) void gh_kv8_attn_l1_k(Kv8AttnArgs a) { attend<1>(a); }
-extern "C" __global__ __launch_bounds__(256) void gh_kv8_attn_l2_k(Kv8AttnArgs a) { attend<2>(a); }
-extern "C" __global__ __launch_bounds__(256) void gh_kv8_attn_l4_k(Kv8AttnArgs a) { attend<4>(a); }
-extern "C" __global__ __launch_bounds__(256) void gh_kv8_attn_l8_k(Kv8AttnArgs a) { attend<8>(a); }
+extern "C" __global__ __launch_bounds__(256, 2) void gh_kv8_attn_l1_k(Kv8AttnArgs a) { attend<1>(a); }
+extern "C" __global__ __launch_bounds__(256, 2) void gh_kv8_attn_l2_k(Kv8AttnArgs a) { attend<2>(a); }
+extern "C" __global__ __launch_bounds__(256, 2) void gh_kv8_attn_l4_k(Kv8AttnArgs a) { attend<4>(a); }
+extern "C" __global__ __launch_bounds__(256, 1) void gh_kv8_attn_l8_k(Kv8AttnArgs a) { attend<8>(a); }
 
-// Joins the splits of a tile, in split order.  grid (tiles * 16 columns, kv heads,
-// sequences), a workgroup a column.
-extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a) {
-  const uint32_t tile = blockIdx.x / KV8_COLS, n = blockIdx.x % KV8_COLS, D = a.c.D, G = a.nq / a.c.nkv;
+// Joins the splits of a tile's column, in split order: the splits' factors in
+// LDS, then a lane a dim.  grid (tiles * columns a tile can have, kv heads, sequences)
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, uint32_t cols) {
+  const uint32_t tile = blockIdx.x / cols, n = blockIdx.x % cols, D = a.c.D;
   Tile t;
   if (!tile_of(a, blockIdx.z, blockIdx.y, tile, &t) || n >= t.ncol) return;
   const uint32_t per = kv8_split_steps(t.steps, a.nsplit, a.chunk);
   if (per >= t.steps) return;  // written by its only split
-  const uint32_t live = (t.steps + per - 1) / per;
-  const uint64_t unit = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / KV8_COLS) + tile;
-  const uint64_t row = KV8_COLS * (uint64_t)(D + 2);
-  const float* p = a.part + unit * a.nsplit * row + n * (uint64_t)(D + 2);
-  float M = -INFINITY, L = 0.f;
-  for (uint32_t s = 0; s < live; s++) M = fmaxf(M, p[s * row + D]);
-  const float base = M == -INFINITY ? 0.f : M;
-  for (uint32_t s = 0; s < live; s++) L += p[s * row + D + 1] * exp2f((p[s * row + D] - base) * kLog2e);
+  const uint32_t live = (t.steps + per - 1) / per, tid = threadIdx.x;
+  const uint64_t unit = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / cols) + tile;
+  const uint64_t row = KV8_COLS * (uint64_t)(D + KV8_PART);
+  const float* p = a.part + unit * a.nsplit * row + n * (uint64_t)(D + KV8_PART);
+  __shared__ float f[KV8_MAX_SPLIT], red[8];
+  float m = -INFINITY, l = 0.f;
+  if (tid < live) {
+    m = p[tid * row + D];
+    l = p[tid * row + D + 1];
+  }
+  float M = m;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+  if ((tid & 63) == 0) red[tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float base = M == -INFINITY ? 0.f : M, w = __builtin_amdgcn_exp2f((m - base) * kLog2e);
+  f[tid] = w;
+  const float L0 = wave_sum(l * w);
+  if ((tid & 63) == 0) red[4 + (tid >> 6)] = L0;
+  __syncthreads();
+  const float L = (red[4] + red[5]) + (red[6] + red[7]);
   const float by = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;
-  const uint32_t col = t.col0 + n;
-  float* out = a.out + ((uint64_t)(t.first + col / G) * a.nq + (uint64_t)t.head * G + col % G) * D;
-  for (uint32_t d = threadIdx.x; d < D; d += 256) {
+  float* out = a.out + row_at(a, t, t.col0 + n);
+  for (uint32_t d = tid; d < D; d += 256) {
     float o = 0.f;
-    for (uint32_t s = 0; s < live; s++) o += p[s * row + d] * exp2f((p[s * row + D] - base) * kLog2e);
+    uint32_t s = 0;
+    for (; s + 8 <= live; s += 8) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = p[(s + i) * row + d];
+#pragma unroll
+      for (int i = 0; i < 8; i++) o = fmaf(x[i], f[s + i], o);
+    }
+    for (; s < live; s++) o = fmaf(p[s * row + d], f[s], o);
     out[d] = o * by;
   }
 }
