@@ -6,7 +6,8 @@
 
 #define KV8_BLOCK 16u      // tokens that share a scale, and rows of one matrix tile
 #define KV8_STEP 32u       // tokens of one step of the attention
-#define KV8_COLS 16u       // query rows of one attention tile
+#define KV8_COLS 16u       // query columns of a wave (a row's heads of one kv head, row after row)
+#define KV8_ROW_COLS 32u   // and of a workgroup of many columns
 #define KV8_MAX_SPLIT 256u // parts of one tile's token range
 #define KV8_PART 4u        // floats of a part's row behind its D sums: maximum, sum, and two unused
 #define KV8_Q_HEADS 4u     // query heads of one append workgroup
@@ -45,7 +46,7 @@ struct Kv8AttnArgs {
   Kv8Rows b;
   const float* q;  // [num_rows][nq D]
   float* out;      // [num_rows][nq D]
-  float* part;     // [tile][split][16 query rows][D + KV8_PART]; unused with one split
+  float* part;     // [tile][split][column][D + KV8_PART]; unused with one split
   uint32_t nq, window, nsplit, chunk;  // chunk: steps of a split at least
   float scale;
 };

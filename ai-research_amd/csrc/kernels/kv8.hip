@@ -27,6 +27,9 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 namespace {
 
+// (uniform to the compiler too)
+__device__ __forceinline__ uint32_t wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // First row and number of rows of sequence s, whatever seq_start holds.
 __device__ __forceinline__ uint32_t seq_rows(const Kv8Rows& b, uint32_t s, uint32_t* first) {
   const uint32_t r0 = min(b.seq_start[s], b.num_rows), r1 = min(b.seq_start[s + 1], b.num_rows);
@@ -42,10 +45,10 @@ __device__ __forceinline__ uint32_t page_of(const Kv8View& c, const Kv8Rows& b, 
   return min(b.pages[(uint64_t)s * b.max_pages + i], c.num_pages);
 }
 
-// Index of (page, head, block) among the cache's blocks.
-__device__ __forceinline__ uint64_t block_at(const Kv8View& c, uint32_t page, uint32_t head, uint64_t blk) {
+// Index of (page, head, block) among the cache's blocks (the host refuses 2^32).
+__device__ __forceinline__ uint32_t block_at(const Kv8View& c, uint32_t page, uint32_t head, uint64_t blk) {
   const uint32_t sh = c.page_shift - 4;
-  return (((uint64_t)page * c.nkv + head) << sh) + (blk & ((1u << sh) - 1u));
+  return ((page * c.nkv + head) << sh) + ((uint32_t)blk & ((1u << sh) - 1u));
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -107,7 +110,7 @@ __device__ void block_angles(Angle* ang, uint64_t pos0, uint32_t nr, uint32_t ro
 
 template <int NP>
 __device__ void append_q(const Kv8AppendArgs& a, const Angle* ang, uint32_t row0, uint32_t nr, uint32_t group) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t lane = threadIdx.x & 63, wave = wave_id();
   const uint32_t D = a.c.D, half = a.rot / 2;
   const uint32_t h0 = group * KV8_Q_HEADS, nh = min(KV8_Q_HEADS, a.nq - h0);
   for (uint32_t t = wave; t < nr * nh; t += 4) {
@@ -152,10 +155,10 @@ __device__ __forceinline__ uint32_t v_place(uint32_t t, uint32_t d, uint32_t D) 
 
 template <int NP, bool IS_K>
 __device__ void append_kv(const Kv8AppendArgs& a, const Angle* ang, int8_t* tile, double* red, uint32_t row0,
-                          uint32_t o0, uint32_t nr, uint32_t head, uint64_t at) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+                          uint32_t o0, uint32_t nr, uint32_t head, uint32_t at) {
+  const uint32_t lane = threadIdx.x & 63, wave = wave_id();
   const uint32_t D = a.c.D, half = a.rot / 2, o1 = o0 + nr;
-  int8_t* codes = (IS_K ? a.c.k : a.c.v) + at * (uint64_t)(KV8_BLOCK * D);
+  int8_t* codes = (IS_K ? a.c.k : a.c.v) + (uint64_t)at * (KV8_BLOCK * D);
   float* scale = (IS_K ? a.c.ks : a.c.vs) + at;
   const float* src = IS_K || a.k_eq_v ? a.k : a.v;
   const float old = o0 > 0 ? *scale : 0.f;
@@ -275,7 +278,7 @@ __device__ __forceinline__ void append(const Kv8AppendArgs& a) {
   if (unit < 2 * nkv) {
     const uint32_t head = unit >> 1, page = page_of(a.c, a.b, seq, blk);
     if (page >= a.c.num_pages) return;  // no page: nothing is kept
-    const uint64_t at = block_at(a.c, page, head, blk);
+    const uint32_t at = block_at(a.c, page, head, blk);
     const uint32_t o0 = (uint32_t)(p0 - blk * KV8_BLOCK);
     if (unit & 1) {
       append_kv<NP, false>(a, ang, tile, red, row0, o0, nr, head, at);
@@ -331,7 +334,7 @@ __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
   return u.v;
 }
 
-// a tile of 16 columns of one kv head of a sequence, and its token range
+// a tile of columns of one kv head of a sequence, and its token range
 struct Tile {
   uint32_t seq, head, first, rows, col0, ncol;
   uint64_t past, lo, hi;  // tokens [lo, hi) are visible to one of its columns
@@ -340,15 +343,16 @@ struct Tile {
 };
 
 // false: the tile has no row
-__device__ __forceinline__ bool tile_of(const Kv8AttnArgs& a, uint32_t seq, uint32_t head, uint32_t tile, Tile* t) {
+__device__ __forceinline__ bool tile_of(const Kv8AttnArgs& a, uint32_t seq, uint32_t head, uint32_t tile, uint32_t width,
+                                        Tile* t) {
   const uint32_t G = a.nq / a.c.nkv;
   t->rows = seq_rows(a.b, seq, &t->first);
   t->seq = seq;
   t->head = head;
-  t->col0 = tile * KV8_COLS;
+  t->col0 = tile * width;
   const uint64_t cols = (uint64_t)t->rows * G;
   if (t->col0 >= cols) return false;
-  t->ncol = (uint32_t)min((uint64_t)KV8_COLS, cols - t->col0);
+  t->ncol = (uint32_t)min((uint64_t)width, cols - t->col0);
   t->past = a.b.past[seq];
   const uint64_t p0 = t->past + t->col0 / G, p1 = t->past + (t->col0 + t->ncol - 1) / G;
   const uint64_t lo = a.window && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
@@ -371,33 +375,40 @@ struct Codes {
   bool has[2];
 };
 
-// The pages of 32 of a wave's steps (s, s + 4, ...), two blocks each, in its lanes.
-__device__ __forceinline__ uint32_t step_pages(const Kv8AttnArgs& a, const Tile& t, uint32_t s) {
+// The pages of 32 steps (s, s + stride, ...), two blocks each, in a wave's lanes.
+__device__ __forceinline__ uint32_t step_pages(const Kv8AttnArgs& a, const Tile& t, uint32_t s, uint32_t stride) {
   const uint32_t lane = threadIdx.x & 63;
-  const uint64_t blk = 2 * ((uint64_t)s + 4 * (lane >> 1)) + (lane & 1);
+  const uint64_t blk = 2 * ((uint64_t)s + stride * (lane >> 1)) + (lane & 1);
   // a block that no column sees may hold anything, scales too
   const bool some = blk * KV8_BLOCK < t.hi && (blk + 1) * KV8_BLOCK > t.lo;
   return some ? page_of(a.c, a.b, t.seq, blk) : a.c.num_pages;
 }
 
-template <int NL, bool IS_K>
+// A lane's 16-byte piece of a block: 16 dims of a token (K), 4 tokens of 4 dims (V),
+// dims 64 l ...  FULL: the head has 64 dims for every l; else pieces of dims it does
+// not have are read from the block's first ones, and meet zeros of Q or are not
+// written.
+template <bool FULL, bool IS_K>
+__device__ __forceinline__ uint32_t piece_at(uint32_t l, uint32_t D) {
+  const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  if (IS_K) return FULL || 64 * l + 16 * g < D ? l * 1024 + lane * 16 : n * 16;
+  return FULL || 64 * l + 4 * n < D ? g * 4 * D + l * 256 + n * 16 : 0;
+}
+
+template <int NL, bool FULL, bool IS_K>
 __device__ __forceinline__ void load_codes(const Kv8AttnArgs& a, const Tile& t, uint32_t step, uint32_t pages, uint32_t i,
                                            Codes<NL>* s) {
-  const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, D = a.c.D;
+  const uint32_t D = FULL ? 64 * NL : a.c.D;
 #pragma unroll
   for (int b = 0; b < 2; b++) {
     const uint64_t blk = (uint64_t)step * 2 + b;
     const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)(2 * i + b));
     s->has[b] = page < a.c.num_pages;
-    const uint64_t at = block_at(a.c, s->has[b] ? page : 0, t.head, blk);
+    const uint32_t at = block_at(a.c, s->has[b] ? page : 0, t.head, blk);
     s->s[b] = (IS_K ? a.c.ks : a.c.vs)[at];
-    const int8_t* c = (IS_K ? a.c.k : a.c.v) + at * (uint64_t)(KV8_BLOCK * D);
+    const int8_t* c = (IS_K ? a.c.k : a.c.v) + (uint64_t)at * (KV8_BLOCK * D);
 #pragma unroll
-    for (int l = 0; l < NL; l++) {
-      s->c[b][l] = i32x4{0, 0, 0, 0};
-      const uint32_t place = IS_K ? (4 * l + g) * 256 + n * 16 : g * 4 * D + (16 * l + n) * 16;
-      if ((IS_K ? 64 * l + 16 * g : 64 * l + 4 * n) < D) s->c[b][l] = *reinterpret_cast<const i32x4*>(c + place);
-    }
+    for (int l = 0; l < NL; l++) s->c[b][l] = *reinterpret_cast<const i32x4*>(c + piece_at<FULL, IS_K>(l, D));
   }
 }
 
@@ -426,52 +437,82 @@ __device__ __forceinline__ float digit_sum(int d3, int d2, int d1, int d0) {
   return fmaf((float)((d3 << 8) + d2), 65536.f, (float)((d1 << 8) + d0));
 }
 
-// The softmax of a step's scores sc (-inf: not seen): the halves of P for the
-// second product, and the running values.
+// Over the four lanes of a column (lane, lane ^ 16, ^ 32, ^ 48).
+__device__ __forceinline__ float column_max(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ float uniform(float x) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
+}
+
+// Two numbers as f16, to nearest.
+__device__ __forceinline__ f16x2 half2(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_convertvector((f32x2{a, b}), f16x2);
+}
+
+// The softmax of a step's scores sc, in units of log2 (-inf: not seen): the halves
+// of P for the second product, and the running values.  vs: the blocks' scales of V.
 template <int NL>
 __device__ __forceinline__ void soft_step(const float (&sc)[2][4], const float (&vs)[2], const bool (&has)[2], Run<NL>* r,
                                           f16x8* phi, f16x8* plo) {
-  float mx = r->m;
+  float mx = r->m, vmul[2];
   int E = r->E;
+  bool odd = false;  // a scale that is no number
 #pragma unroll
   for (int b = 0; b < 2; b++) {
 #pragma unroll
     for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[b][i]);
-    // the exponent of a scale that counts (a power of two; 0 and NaN have none)
-    if (has[b] && vs[b] > 0.f && vs[b] < INFINITY) E = max(E, (int)((__float_as_uint(vs[b]) >> 23) & 255) - 127);
+    // the exponent of a scale that counts (a power of two; 0 has none)
+    const uint32_t bits = __builtin_amdgcn_readfirstlane(__float_as_uint(vs[b]));
+    const bool number = bits - 1u < 0x7f800000u - 1u;
+    odd |= has[b] && bits >= 0x7f800000u;
+    if (has[b] && number) E = max(E, (int)(bits >> 23) - 127);
   }
-  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  mx = column_max(mx);
   const float base = mx == -INFINITY ? 0.f : mx;
-  const float alpha = __builtin_amdgcn_exp2f((r->m - base) * kLog2e);
+  const float alpha = __builtin_amdgcn_exp2f(r->m - base);
   const float turn = r->E == E ? alpha : alpha * ldexpf(1.f, max(r->E - E, -200));
   r->m = mx;
   r->E = E;
-  union {
-    _Float16 h[8];
-    f16x8 v;
-  } hi, lo;
-  float sum = 0.f;
 #pragma unroll
-  for (int b = 0; b < 2; b++) {
-    const float vmul = ldexpf(vs[b], E == kNoExp ? 0 : 14 - E);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const bool seen = sc[b][i] != -INFINITY;  // (a NaN score is seen)
-      const float p = __builtin_amdgcn_exp2f((sc[b][i] - base) * kLog2e);
-      sum += p;
-      const float w = seen ? p * vmul : 0.f;
-      hi.h[4 * b + i] = (_Float16)w;
-      lo.h[4 * b + i] = (_Float16)(w - (float)hi.h[4 * b + i]);
-    }
-  }
-  r->l = r->l * alpha + sum;
+  for (int b = 0; b < 2; b++) vmul[b] = has[b] ? ldexpf(vs[b], E == kNoExp ? 0 : 14 - E) : 0.f;
   if (__any(turn != 1.f)) {
 #pragma unroll
     for (int l = 0; l < NL; l++)
 #pragma unroll
       for (int j = 0; j < 4; j++) r->o[l][j] *= turn;
   }
+  union {
+    f16x2 h[4];
+    f16x8 v;
+  } hi, lo;
+  float sum = 0.f;
+#pragma unroll
+  for (int b = 0; b < 2; b++) {
+    float w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float p = __builtin_amdgcn_exp2f(sc[b][i] - base);
+      sum += p;
+      w[i] = p * vmul[b];
+    }
+    if (odd) {  // (a NaN score is seen)
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[i] = sc[b][i] != -INFINITY ? w[i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const f16x2 h = half2(w[2 * i], w[2 * i + 1]);
+      hi.h[2 * b + i] = h;
+      lo.h[2 * b + i] = half2(w[2 * i] - (float)h[0], w[2 * i + 1] - (float)h[1]);
+    }
+  }
+  r->l = r->l * alpha + sum;
   *phi = hi.v;
   *plo = lo.v;
 }
@@ -481,11 +522,44 @@ __device__ __forceinline__ bool visible(int64_t t, int64_t pos, uint32_t window)
   return t <= pos && (window == 0 || t > pos - (int64_t)window);
 }
 
-// Scores of a step's tokens 4 g .. of both blocks for a lane's column; -inf: not seen.
+// The digit sums are used behind a branch: the compiler (ROCm 7.2) counts the eight
+// wait states from a matrix instruction to a read of its result within a block,
+// and put the read right behind the branch of one that ended with the products.
+__device__ __forceinline__ void settle(i32x4 (&acc)[2][4]) {
+  asm volatile("s_nop 7"
+               : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[0][2]), "+v"(acc[0][3]), "+v"(acc[1][0]), "+v"(acc[1][1]),
+                 "+v"(acc[1][2]), "+v"(acc[1][3]));
+}
+
+// Scores, in units of log2, from their digit sums; -inf: not seen.
+__device__ __forceinline__ void finish_scores(const Kv8AttnArgs& a, i32x4 (&acc)[2][4], const float (&ks)[2],
+                                              const bool (&has)[2], float qmul, const Tile& t, int64_t pos, uint32_t step,
+                                              float (&sc)[2][4]) {
+  const uint32_t g = (threadIdx.x & 63) >> 4;
+  settle(acc);
+#pragma unroll
+  for (int b = 0; b < 2; b++) {
+    const float mul = qmul * ks[b];  // (powers of two and the constant: one rounding, of the constant)
+#pragma unroll
+    for (int i = 0; i < 4; i++) sc[b][i] = digit_sum(acc[b][3][i], acc[b][2][i], acc[b][1][i], acc[b][0][i]) * mul;
+  }
+  // every token of the step is seen by every column
+  const bool whole = has[0] && has[1] && (uint64_t)step * KV8_STEP >= t.all_lo && ((uint64_t)step + 1) * KV8_STEP <= t.all_hi;
+  if (!whole) {
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const int64_t t0 = (int64_t)step * KV8_STEP + b * KV8_BLOCK + 4 * g;
+#pragma unroll
+      for (int i = 0; i < 4; i++) sc[b][i] = has[b] && visible(t0 + i, pos, a.window) ? sc[b][i] : -INFINITY;
+    }
+  }
+}
+
+// Scores of a step's tokens 4 g .. of both blocks for a lane's column.
 template <int NL>
 __device__ __forceinline__ void score_step(const Kv8AttnArgs& a, const Codes<NL>& k, const i32x4* qd, float qmul,
                                            const Tile& t, int64_t pos, uint32_t step, float (&sc)[2][4]) {
-  const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
+  const uint32_t lane = threadIdx.x & 63;
   i32x4 acc[2][4];
   asm volatile("" ::: "memory");  // the digits are read in every step, not held
 #pragma unroll
@@ -499,19 +573,7 @@ __device__ __forceinline__ void score_step(const Kv8AttnArgs& a, const Codes<NL>
       acc[1][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k.c[1][l], q, acc[1][d], 0, 0, 0);
     }
   }
-  // every token of the step is seen by every column
-  const bool whole = k.has[0] && k.has[1] && (uint64_t)step * KV8_STEP >= t.all_lo && ((uint64_t)step + 1) * KV8_STEP <= t.all_hi;
-#pragma unroll
-  for (int b = 0; b < 2; b++) {
-    const float mul = qmul * k.s[b];
-#pragma unroll
-    for (int i = 0; i < 4; i++) sc[b][i] = digit_sum(acc[b][3][i], acc[b][2][i], acc[b][1][i], acc[b][0][i]) * mul * a.scale;
-    if (!whole) {
-      const int64_t t0 = (int64_t)step * KV8_STEP + b * KV8_BLOCK + 4 * g;
-#pragma unroll
-      for (int i = 0; i < 4; i++) sc[b][i] = k.has[b] && visible(t0 + i, pos, a.window) ? sc[b][i] : -INFINITY;
-    }
-  }
+  finish_scores(a, acc, k.s, k.has, qmul, t, pos, step, sc);
 }
 
 template <int NL>
@@ -547,6 +609,51 @@ __device__ __forceinline__ void digits4(const int (&v)[4], int (&w)[4]) {
   w[3] = (int)__builtin_amdgcn_perm(b1, a1, 0x07060302u);
 }
 
+// A lane's part of its column's query row (dims 64 l + 16 g ..) as digits; the row's
+// largest magnitude decides their unit, which is returned (NaN where the row has a
+// NaN or an infinity).
+template <int NL>
+__device__ __forceinline__ float load_q(const Kv8AttnArgs& a, const float* q, i32x4 (&qd)[4][NL]) {
+  const uint32_t g = (threadIdx.x & 63) >> 4, D = a.c.D;
+  f32x4 x[NL][4];
+  float amax = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int l = 0; l < NL; l++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      x[l][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (64 * l + 16 * g < D) x[l][j] = *reinterpret_cast<const f32x4*>(q + 64 * l + 16 * g + 4 * j);
+    }
+#pragma unroll
+  for (int l = 0; l < NL; l++)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        amax = fmaxf(amax, fabsf(x[l][j][i]));
+        bad |= !(fabsf(x[l][j][i]) < INFINITY);
+      }
+  if (bad) amax = INFINITY;
+  amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+  amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+  bad = amax == INFINITY;
+  int e = 0;
+  if (!bad) frexpf(amax, &e);
+#pragma unroll
+  for (int l = 0; l < NL; l++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      int v[4], w[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = bad ? 0 : (int)rintf(ldexpf(x[l][j][i], 30 - e));
+      digits4(v, w);
+#pragma unroll
+      for (int d = 0; d < 4; d++) qd[d][l][j] = w[d];
+    }
+  return bad ? __builtin_nanf("") : ldexpf(1.f, e - 30);
+}
+
 // The tile's query columns as digits in LDS, qd[digit][l][lane] (dims 64 l + 16 g
 // .. of column n); a wave makes every fourth l.  A row's largest magnitude (joined
 // through qm) decides its unit, which is returned (NaN where the row has a NaN or
@@ -554,7 +661,7 @@ __device__ __forceinline__ void digits4(const int (&v)[4], int (&w)[4]) {
 template <int NL>
 __device__ __forceinline__ float stage_q(const Kv8AttnArgs& a, const float* q, float* qm, i32x4* qd) {
   constexpr int NS = (NL + 3) / 4;
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4, D = a.c.D;
+  const uint32_t lane = threadIdx.x & 63, wave = wave_id(), n = lane & 15, g = lane >> 4, D = a.c.D;
   f32x4 x[NS][4];
   float amax = 0.f;
   bool bad = false;
@@ -606,19 +713,32 @@ __device__ __forceinline__ float stage_q(const Kv8AttnArgs& a, const float* q, f
   return bad ? __builtin_nanf("") : ldexpf(1.f, e - 30);
 }
 
+// A lane's sums of its column (dims 64 l + 16 g + 4 i .. for each l, i), times by.
+template <int NL>
+__device__ __forceinline__ void write_column(const Run<NL>& r, float* to, uint32_t D, float by) {
+  const uint32_t g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int l = 0; l < NL; l++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t d = 64 * l + 16 * g + 4 * i;
+      if (d < D) *reinterpret_cast<f32x4*>(to + d) = f32x4{r.o[l][0][i], r.o[l][1][i], r.o[l][2][i], r.o[l][3][i]} * by;
+    }
+}
+
 // Few query columns (one tile): the workgroup's waves take its steps in turn.  The
 // tokens' bytes bound it, so a wave has the next step's keys on the way while it
 // weighs this step's values, and the next values while it scores; the query
 // digits are in LDS to leave the registers to them.
 // grid (tiles * splits, kv heads, sequences)
-template <int NL>
+template <int NL, bool FULL>
 __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   extern __shared__ __align__(16) char lds[];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const uint32_t lane = threadIdx.x & 63, wave = wave_id(), n = lane & 15, g = lane >> 4;
   const uint32_t D = a.c.D, G = a.nq / a.c.nkv;
   const uint32_t split = blockIdx.x % a.nsplit, tile = blockIdx.x / a.nsplit;
   Tile t;
-  if (!tile_of(a, blockIdx.z, blockIdx.y, tile, &t)) return;
+  if (!tile_of(a, blockIdx.z, blockIdx.y, tile, KV8_COLS, &t)) return;
   const uint32_t per = kv8_split_steps(t.steps, a.nsplit, a.chunk);
   const uint32_t s0 = t.step0 + split * per, end = t.step0 + t.steps;
   if (split > 0 && s0 >= end) return;
@@ -628,16 +748,16 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   float* ll = lm + 64;                               // [4][16]
   i32x4* qd = reinterpret_cast<i32x4*>(lds + 512);   // [4][NL][64]
   float* lo = reinterpret_cast<float*>(lds + 512);   // [2 waves][16 NL floats][64 lanes], after the steps
-  uint32_t pages = step_pages(a, t, s0 + wave);
+  uint32_t pages = step_pages(a, t, s0 + wave, 4);
   const uint32_t col = t.col0 + min(n, t.ncol - 1);  // columns past the last repeat it
   const int64_t pos = (int64_t)(t.past + col / G);
   Codes<NL> k, v;
   uint32_t i = 0, s = s0 + wave;
   if (s < s1) {
-    load_codes<NL, true>(a, t, s, pages, 0, &k);
-    load_codes<NL, false>(a, t, s, pages, 0, &v);
+    load_codes<NL, FULL, true>(a, t, s, pages, 0, &k);
+    load_codes<NL, FULL, false>(a, t, s, pages, 0, &v);
   }
-  const float qmul = stage_q<NL>(a, a.q + row_at(a, t, col), lm, qd);
+  const float qmul = stage_q<NL>(a, a.q + row_at(a, t, col), lm, qd) * (a.scale * kLog2e);
   Run<NL> r;
   clear<NL>(&r);
   for (; s < s1; s += 4) {
@@ -646,14 +766,14 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
     const bool more = s + 4 < s1;
     if (++i == 32 && more) {
       i = 0;
-      pages = step_pages(a, t, s + 4);
+      pages = step_pages(a, t, s + 4, 4);
     }
-    if (more) load_codes<NL, true>(a, t, s + 4, pages, i, &k);
+    if (more) load_codes<NL, FULL, true>(a, t, s + 4, pages, i, &k);
     __builtin_amdgcn_sched_barrier(0);
     f16x8 hi, lo;
     soft_step<NL>(sc, v.s, v.has, &r, &hi, &lo);
     value_step<NL>(v, hi, lo, &r);
-    if (more) load_codes<NL, false>(a, t, s + 4, pages, i, &v);
+    if (more) load_codes<NL, FULL, false>(a, t, s + 4, pages, i, &v);
     __builtin_amdgcn_sched_barrier(0);
   }
   r.l += __shfl_xor(r.l, 16, 64);
@@ -670,8 +790,8 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   for (int w = 0; w < 4; w++) M = fmaxf(M, lm[w * 16 + n]);
   const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
-  for (int w = 0; w < 4; w++) L += ll[w * 16 + n] * __builtin_amdgcn_exp2f((lm[w * 16 + n] - base) * kLog2e);
-  const float f = __builtin_amdgcn_exp2f((r.m - base) * kLog2e), fe = r.E == kNoExp ? 0.f : ldexpf(f, r.E - 14);
+  for (int w = 0; w < 4; w++) L += ll[w * 16 + n] * __builtin_amdgcn_exp2f(lm[w * 16 + n] - base);
+  const float f = __builtin_amdgcn_exp2f(r.m - base), fe = r.E == kNoExp ? 0.f : ldexpf(f, r.E - 14);
 #pragma unroll
   for (int l = 0; l < NL; l++)
 #pragma unroll
@@ -714,13 +834,193 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
       to[D + 1] = L;
     }
   }
+  write_column<NL>(r, to, D, by);
+}
+
+// Many query columns (a prompt's).  The matrix instructions bound it (per step and
+// 16 columns of 256 dims 64 of them, 1024 cycles of a SIMD), as far as the vector
+// ones run beside them: two workgroups a CU, which no barrier couples, give every
+// SIMD two waves for that.  A workgroup takes 32 columns: waves 0 and 1 sixteen each
+// for the even steps, waves 2 and 3 the same for the odd ones, joined at the end,
+// so that the workgroups of a causal prompt are short and many enough to even out
+// over the CUs (64 columns over all steps: the longest takes as long as the rest
+// together).  The codes of a step come through LDS once for its two waves, the values'
+// already as f16, whose conversion is as much vector work as the softmax; the next
+// step's are on their way to registers meanwhile.
+// grid (tiles * splits * kv heads, 1, sequences), the tiles that see most first; the
+// heads in turn, so that with eight of them a head's workgroups share an XCD's L2.
+template <int NL, bool FULL>
+__device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int NS = (NL + 1) / 2;
+  constexpr uint32_t kPieces = 2 * NL * 64, vPieces = 4 * NL * 64;  // 16 bytes each, of a step
+  const uint32_t lane = threadIdx.x & 63, wave = wave_id(), n = lane & 15, g = lane >> 4;
+  const uint32_t part = wave & 1, par = wave >> 1;
+  const uint32_t D = FULL ? 64 * NL : a.c.D, G = a.nq / a.c.nkv, each = a.c.nkv * a.nsplit, tiles = gridDim.x / each;
+  const uint32_t head = blockIdx.x % a.c.nkv, split = blockIdx.x / a.c.nkv % a.nsplit, tile = tiles - 1 - blockIdx.x / each;
+  Tile t;
+  if (!tile_of(a, blockIdx.z, head, tile, KV8_ROW_COLS, &t)) return;
+  const uint32_t per = kv8_split_steps(t.steps, a.nsplit, a.chunk);
+  const uint32_t s0 = t.step0 + split * per, end = t.step0 + t.steps;
+  if (split > 0 && s0 >= end) return;
+  const uint32_t s1 = min(s0 + per, end);
+  i32x4* kb = reinterpret_cast<i32x4*>(lds) + par * (kPieces + vPieces);
+  f16x8* vb = reinterpret_cast<f16x8*>(kb + kPieces);
+
+  // this wave's columns (past the last they repeat it), and what they see
+  const uint32_t c0 = t.col0 + part * KV8_COLS, last = t.col0 + t.ncol - 1, col = min(c0 + n, last);
+  const int64_t pos = (int64_t)(t.past + col / G);
+  Tile mine = t;
+  {
+    const uint64_t p0 = t.past + min(c0, last) / G, p1 = t.past + min(c0 + KV8_COLS - 1, last) / G;
+    mine.lo = a.window && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
+    mine.hi = p1 + 1;
+    mine.all_lo = a.window && p1 + 1 > a.window ? p1 + 1 - a.window : 0;
+    mine.all_hi = p0 + 1;
+  }
+
+  uint32_t pages = step_pages(a, t, s0 + par, 2), at = 0;
+  i32x4 kc[2][NS], vc[2][NS];
+  float ks[2], vs[2], ks_next[2], vs_next[2];
+  bool has[2], has_next[2];
+  const auto load = [&](uint32_t step) {
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const uint64_t blk = (uint64_t)step * 2 + b;
+      const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)(2 * at + b));
+      has_next[b] = page < a.c.num_pages;
+      const uint32_t place = block_at(a.c, has_next[b] ? page : 0, t.head, blk);
+      ks_next[b] = a.c.ks[place];
+      vs_next[b] = a.c.vs[place];
+      const int8_t* k = a.c.k + (uint64_t)place * (KV8_BLOCK * D);
+      const int8_t* v = a.c.v + (uint64_t)place * (KV8_BLOCK * D);
+#pragma unroll
+      for (int i = 0; i < NS; i++) {
+        const uint32_t l = NL == 1 ? 0 : part + 2 * i;
+        kc[b][i] = *reinterpret_cast<const i32x4*>(k + piece_at<FULL, true>(l, D));
+        vc[b][i] = *reinterpret_cast<const i32x4*>(v + piece_at<FULL, false>(l, D));
+      }
+    }
+    if (++at == 32) {
+      at = 0;
+      pages = step_pages(a, t, step + 2, 2);
+    }
+  };
+  const auto store = [&]() {
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+      const uint32_t l = NL == 1 ? 0 : part + 2 * i;
+#pragma unroll
+      for (int b = 0; b < 2; b++) kb[(b * NL + l) * 64 + lane] = kc[b][i];
+#pragma unroll
+      for (int j = 0; j < 4; j++) vb[(l * 4 + j) * 64 + lane] = codes_f16((uint32_t)vc[0][i][j], (uint32_t)vc[1][i][j]);
+    }
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      ks[b] = ks_next[b];
+      vs[b] = vs_next[b];
+      has[b] = has_next[b];
+    }
+  };
+
+  i32x4 qd[4][NL];
+  uint32_t s = s0 + par;
+  if (s < s1) load(s);
+  const float qmul = load_q<NL>(a, a.q + row_at(a, t, col), qd) * (a.scale * kLog2e);
+  // the lowest digits are in LDS: the registers hold three of four
+  i32x4* q0 = reinterpret_cast<i32x4*>(lds) + 2 * (kPieces + vPieces) + part * NL * 64;
+  if (par == 0) {
+#pragma unroll
+    for (int l = 0; l < NL; l++) q0[l * 64 + lane] = qd[0][l];
+  }
+  Run<NL> r;
+  clear<NL>(&r);
+  for (uint32_t first = s0; first < s1; first += 2, s += 2) {
+    if (s < s1) store();
+    if (s + 2 < s1) load(s + 2);
+    __syncthreads();
+    // (a step that none of the wave's columns sees: the others' barriers only)
+    if (s < s1 && (uint64_t)s * KV8_STEP < mine.hi && ((uint64_t)s + 1) * KV8_STEP > mine.lo) {
+      float sc[2][4];
+      {
+        i32x4 acc[2][4];
+#pragma unroll
+        for (int d = 0; d < 4; d++) acc[0][d] = acc[1][d] = i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int l = 0; l < NL; l++) {
+          const i32x4 k0 = kb[l * 64 + lane], k1 = kb[(NL + l) * 64 + lane], low = q0[l * 64 + lane];
+#pragma unroll
+          for (int d = 0; d < 4; d++) {
+            const i32x4 q = d == 0 ? low : qd[d][l];
+            acc[0][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k0, q, acc[0][d], 0, 0, 0);
+            acc[1][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k1, q, acc[1][d], 0, 0, 0);
+          }
+        }
+        finish_scores(a, acc, ks, has, qmul, mine, pos, s, sc);
+      }
+      f16x8 x[4];  // the values' operands, one l ahead
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[j] = vb[j * 64 + lane];
+      f16x8 hi, lo;
+      soft_step<NL>(sc, vs, has, &r, &hi, &lo);
+#pragma unroll
+      for (int l = 0; l < NL; l++) {
+        f16x8 y[4];
+        if (l + 1 < NL) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) y[j] = vb[((l + 1) * 4 + j) * 64 + lane];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) r.o[l][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[j], hi, r.o[l][j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; j++) r.o[l][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[j], lo, r.o[l][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = y[j];
+      }
+    }
+    __syncthreads();
+  }
+  r.l += __shfl_xor(r.l, 16, 64);
+  r.l += __shfl_xor(r.l, 32, 64);
+  // the odd steps' sums come to the wave of the even ones
+  float unit = r.E == kNoExp ? 0.f : ldexpf(1.f, r.E - 14);
+  float* lm = reinterpret_cast<float*>(lds) + part * (16 * NL * 64 + 128);
+  float* lo = lm + 128;
+  if (par == 1) {
+    lm[lane] = r.m;
+    lm[64 + lane] = r.l;
+#pragma unroll
+    for (int l = 0; l < NL; l++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) lo[(l * 16 + j * 4 + i) * 64 + lane] = r.o[l][j][i] * unit;
+  }
+  __syncthreads();
+  if (par == 1) return;
+  const float m1 = lm[lane], M = fmaxf(r.m, m1), base = M == -INFINITY ? 0.f : M;
+  const float f0 = __builtin_amdgcn_exp2f(r.m - base), f1 = __builtin_amdgcn_exp2f(m1 - base);
+  const float L = r.l * f0 + lm[64 + lane] * f1;
+  unit *= f0;
 #pragma unroll
   for (int l = 0; l < NL; l++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t d = 64 * l + 16 * g + 4 * i;
-      if (d < D) *reinterpret_cast<f32x4*>(to + d) = f32x4{r.o[l][0][i], r.o[l][1][i], r.o[l][2][i], r.o[l][3][i]} * by;
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) r.o[l][j][i] = fmaf(lo[(l * 16 + j * 4 + i) * 64 + lane], f1, r.o[l][j][i] * unit);
+  if (c0 + n > last) return;
+  if (per >= t.steps) {  // the only split that runs; nothing visible: 0
+    write_column<NL>(r, a.out + row_at(a, t, col), D, M == -INFINITY && L == 0.f ? 0.f : 1.f / L);
+  } else {
+    const uint64_t place = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * tiles + tile;
+    float* to = a.part + ((place * a.nsplit + split) * KV8_ROW_COLS + (col - t.col0)) * (D + KV8_PART);
+    if (g == 0) {
+      to[D] = M;
+      to[D + 1] = L;
     }
+    write_column<NL>(r, to, D, 1.f);
+  }
 }
 
 }  // namespace
@@ -729,22 +1029,28 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_append_p1_k(Kv8AppendAr
 extern "C" __global__ __launch_bounds__(256) void gh_kv8_append_p2_k(Kv8AppendArgs a) { append<2>(a); }
 extern "C" __global__ __launch_bounds__(256) void gh_kv8_append_p4_k(Kv8AppendArgs a) { append<4>(a); }
 
-extern "C" __global__ __launch_bounds__(256, 2) void gh_kv8_attn_l1_k(Kv8AttnArgs a) { attend<1>(a); }
-extern "C" __global__ __launch_bounds__(256, 2) void gh_kv8_attn_l2_k(Kv8AttnArgs a) { attend<2>(a); }
-extern "C" __global__ __launch_bounds__(256, 2) void gh_kv8_attn_l4_k(Kv8AttnArgs a) { attend<4>(a); }
-extern "C" __global__ __launch_bounds__(256, 1) void gh_kv8_attn_l8_k(Kv8AttnArgs a) { attend<8>(a); }
+#define KV8_ATTN(NL, WAVES)                                                                                       \
+  extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_attn_l##NL##_k(Kv8AttnArgs a) { attend<NL, true>(a); } \
+  extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_attn_l##NL##r_k(Kv8AttnArgs a) { attend<NL, false>(a); } \
+  extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_rows_l##NL##_k(Kv8AttnArgs a) { attend_rows<NL, true>(a); } \
+  extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_rows_l##NL##r_k(Kv8AttnArgs a) { attend_rows<NL, false>(a); }
+KV8_ATTN(1, 2)
+KV8_ATTN(2, 2)
+KV8_ATTN(4, 2)
+KV8_ATTN(8, 1)
 
 // Joins the splits of a tile's column, in split order: the splits' factors in
 // LDS, then a lane a dim.  grid (tiles * columns a tile can have, kv heads, sequences)
-extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, uint32_t cols) {
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, uint32_t width,
+                                                                           uint32_t cols) {
   const uint32_t tile = blockIdx.x / cols, n = blockIdx.x % cols, D = a.c.D;
   Tile t;
-  if (!tile_of(a, blockIdx.z, blockIdx.y, tile, &t) || n >= t.ncol) return;
+  if (!tile_of(a, blockIdx.z, blockIdx.y, tile, width, &t) || n >= t.ncol) return;
   const uint32_t per = kv8_split_steps(t.steps, a.nsplit, a.chunk);
   if (per >= t.steps) return;  // written by its only split
   const uint32_t live = (t.steps + per - 1) / per, tid = threadIdx.x;
   const uint64_t unit = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / cols) + tile;
-  const uint64_t row = KV8_COLS * (uint64_t)(D + KV8_PART);
+  const uint64_t row = width * (uint64_t)(D + KV8_PART);
   const float* p = a.part + unit * a.nsplit * row + n * (uint64_t)(D + KV8_PART);
   __shared__ float f[KV8_MAX_SPLIT], red[8];
   float m = -INFINITY, l = 0.f;
@@ -758,7 +1064,7 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, 
   if ((tid & 63) == 0) red[tid >> 6] = M;
   __syncthreads();
   M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float base = M == -INFINITY ? 0.f : M, w = __builtin_amdgcn_exp2f((m - base) * kLog2e);
+  const float base = M == -INFINITY ? 0.f : M, w = __builtin_amdgcn_exp2f(m - base);
   f[tid] = w;
   const float L0 = wave_sum(l * w);
   if ((tid & 63) == 0) red[4 + (tid >> 6)] = L0;
@@ -794,7 +1100,7 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_read_k(Kv8ReadArgs a) {
   const uint64_t row0 = first + (p0 - past), kv = (uint64_t)a.c.nkv * D;
   const uint32_t page = page_of(a.c, a.b, seq, blk);
   const bool has = page < a.c.num_pages;
-  const uint64_t at = block_at(a.c, has ? page : 0, head, blk);
+  const uint32_t at = block_at(a.c, has ? page : 0, head, blk);
   union Piece {
     int4 w;
     int8_t b[16];
@@ -806,7 +1112,7 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_read_k(Kv8ReadArgs a) {
     const uint32_t j = is_k ? i : i - D;
     Piece p;
     p.w = int4{0, 0, 0, 0};
-    if (has) p.w = reinterpret_cast<const int4*>((is_k ? a.c.k : a.c.v) + at * (uint64_t)(KV8_BLOCK * D))[j];
+    if (has) p.w = reinterpret_cast<const int4*>((is_k ? a.c.k : a.c.v) + (uint64_t)at * (KV8_BLOCK * D))[j];
     const float s = has ? (is_k ? a.c.ks : a.c.vs)[at] : 0.f;
     if (is_k) {
       const uint32_t t = j & 15, d = (j >> 4) * 16;

@@ -56,6 +56,8 @@ gh_status check_cache(const char* who, const gh_kv8_cache* c, Kv8View* v) {
   if (c->num_kv > 4096) return unsupported(who, "more than 4096 kv heads");
   if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
     return invalid(who, "cache codes must be 16-byte aligned, scales 4-byte");
+  if ((uint64_t)c->num_pages * c->num_kv * (c->page_tokens / KV8_BLOCK) >= 1ull << 32)
+    return unsupported(who, "the cache has 2^32 blocks or more");
   uint32_t shift = 4;
   while ((1u << shift) < c->page_tokens) shift++;
   *v = Kv8View{static_cast<int8_t*>(c->k), static_cast<int8_t*>(c->v), c->k_scale, c->v_scale, c->num_pages, shift,
@@ -83,7 +85,8 @@ bool empty(const Kv8Rows& r) { return r.num_seqs == 0 || r.num_rows == 0 || r.ma
 uint32_t touched(const Kv8Rows& r) { return (r.max_rows + KV8_BLOCK - 2) / KV8_BLOCK + 1; }
 
 struct AttnPlan {
-  uint32_t tiles = 0, nsplit = 1, chunk = 4;
+  bool rows = false;  // the kernel of many columns
+  uint32_t width = KV8_COLS, tiles = 0, nsplit = 1, chunk = 4;
   size_t bytes = 0;
 };
 
@@ -99,18 +102,23 @@ gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, co
   if (num_q > 65536) return unsupported(who, "more than 65536 query heads");
   *p = AttnPlan{};
   if (empty(r)) return GH_OK;
-  const uint64_t G = num_q / c.nkv, tiles = (r.max_rows * G + KV8_COLS - 1) / KV8_COLS;
+  const uint64_t G = num_q / c.nkv, cols = r.max_rows * G;
+  static const uint64_t row_min = getenv("KV8_ROWMIN") ? atoi(getenv("KV8_ROWMIN")) : 33;
+  p->rows = cols >= row_min;
+  if (p->rows) p->width = KV8_ROW_COLS;
+  if (p->rows) p->chunk = getenv("KV8_CHUNK") ? atoi(getenv("KV8_CHUNK")) : 16;
+  const uint64_t tiles = (cols + p->width - 1) / p->width;
   uint64_t tokens = (uint64_t)r.max_pages << c.page_shift;
   if (max_kv) tokens = std::min<uint64_t>(tokens, max_kv);
-  if (window) tokens = std::min<uint64_t>(tokens, (uint64_t)window + (KV8_COLS + G - 1) / G);
+  if (window) tokens = std::min<uint64_t>(tokens, (uint64_t)window + (p->width + G - 1) / G);
   const uint64_t steps = tokens / KV8_STEP + 1, units = tiles * c.nkv * r.num_seqs;
   const uint64_t most = std::min<uint64_t>((steps + p->chunk - 1) / p->chunk, KV8_MAX_SPLIT);
-  const uint64_t want = (2ull * ctx->num_cus + units - 1) / units;
+  const uint64_t want = p->rows ? 2ull * ctx->num_cus / units : (2ull * ctx->num_cus + units - 1) / units;
   p->nsplit = (uint32_t)std::max<uint64_t>(1, std::min(want, most));
   p->chunk = (uint32_t)std::max<uint64_t>(p->chunk, (steps + p->nsplit - 1) / p->nsplit);
-  if (tiles * p->nsplit > 0x7fffffffull) return unsupported(who, "too many query rows");
+  if (tiles * p->nsplit * c.nkv > 0x7fffffffull || tiles * p->width > 0x7fffffffull) return unsupported(who, "too many query rows");
   p->tiles = (uint32_t)tiles;
-  if (p->nsplit > 1) p->bytes = (size_t)units * p->nsplit * KV8_COLS * (c.D + KV8_PART) * sizeof(float);
+  if (p->nsplit > 1) p->bytes = (size_t)units * p->nsplit * p->width * (c.D + KV8_PART) * sizeof(float);
   return GH_OK;
 }
 
@@ -242,15 +250,15 @@ gh_status gh_kv8_attn(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8_b
     a.chunk = p.chunk;
     a.scale = scale;
     const uint32_t nl = a.c.D <= 64 ? 1 : a.c.D <= 128 ? 2 : a.c.D <= 256 ? 4 : 8;
-    const char* name = nl == 1   ? "gh_kv8_attn_l1_k"
-                       : nl == 2 ? "gh_kv8_attn_l2_k"
-                       : nl == 4 ? "gh_kv8_attn_l4_k"
-                                 : "gh_kv8_attn_l8_k";
+    // r: heads of fewer dims than the kernel's 64 nl
+    const std::string name = std::string(p.rows ? "gh_kv8_rows_l" : "gh_kv8_attn_l") + std::to_string(nl) +
+                             (a.c.D == 64 * nl ? "_k" : "r_k");
     void* args[] = {&a};
-    st = launch(ctx, name, dim3(p.tiles * p.nsplit, a.c.nkv, a.b.num_seqs), dim3(256), 512 + 8192 * nl, args);
+    st = p.rows ? launch(ctx, name.c_str(), dim3(p.tiles * p.nsplit * a.c.nkv, 1, a.b.num_seqs), dim3(256), 14336 * nl, args)
+                : launch(ctx, name.c_str(), dim3(p.tiles * p.nsplit, a.c.nkv, a.b.num_seqs), dim3(256), 512 + 8192 * nl, args);
     if (st != GH_OK || p.nsplit == 1) return st;
-    uint32_t cols = (uint32_t)std::min<uint64_t>(KV8_COLS, (uint64_t)a.b.max_rows * (num_q / a.c.nkv));
-    void* margs[] = {&a, &cols};
+    uint32_t cols = (uint32_t)std::min<uint64_t>(p.width, (uint64_t)a.b.max_rows * (num_q / a.c.nkv));
+    void* margs[] = {&a, &p.width, &cols};
     return launch(ctx, "gh_kv8_merge_k", dim3(p.tiles * cols, a.c.nkv, a.b.num_seqs), dim3(256), 0, margs);
   });
 }
