@@ -32,13 +32,15 @@ struct Kv8AppendArgs {
   float* qo;                         // [num_rows][nq D]
   uint64_t qs, kvs;
   uint32_t nq, rot, k_eq_v;
-  float theta, eps;
+  float eps;
+  double log_hi, log_lo;  // -2 log2(theta) / rot as the sum of two
 };
 
 struct Kv8ReadArgs {
   Kv8View c;
   Kv8Rows b;
   float *k, *v;  // [num_rows][nkv D], either may be null
+  uint32_t wide;  // both 16-byte aligned
 };
 
 struct Kv8AttnArgs {

@@ -51,11 +51,6 @@ __device__ __forceinline__ uint32_t block_at(const Kv8View& c, uint32_t page, ui
   return ((page * c.nkv + head) << sh) + ((uint32_t)blk & ((1u << sh) - 1u));
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
-}
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
@@ -63,8 +58,49 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 __device__ __forceinline__ double wave_max(double v) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = fmax(v, __shfl_xor(v, off, 64));
+  for (int off = 32; off > 0; off >>= 1) {
+    const double u = __shfl_xor(v, off, 64);
+    v = u > v ? u : v;
+  }
   return v;
+}
+
+// The wave's sums of N values (a power of two) at once: lane l gets that of value l
+// mod N.  While there are several, lanes exchange halves of them.
+template <int N, typename T>
+__device__ __forceinline__ T wave_sums(T (&v)[N]) {
+  const uint32_t lane = threadIdx.x & 63;
+  int bit = 1;
+#pragma unroll
+  for (int n = N; n > 1; n >>= 1, bit <<= 1) {
+#pragma unroll
+    for (int i = 0; i < n / 2; i++) {
+      const bool odd = lane & bit;
+      const T keep = odd ? v[2 * i + 1] : v[2 * i], give = odd ? v[2 * i] : v[2 * i + 1];
+      v[i] = keep + __shfl_xor(give, bit, 64);
+    }
+  }
+#pragma unroll
+  for (int off = N; off < 64; off <<= 1) v[0] += __shfl_xor(v[0], off, 64);
+  return v[0];
+}
+
+// Lane l's value, in every lane.
+__device__ __forceinline__ float lane_value(float v, int l) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l));
+}
+__device__ __forceinline__ double lane_value(double v, int l) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, l), hi = (uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), l);
+  return __longlong_as_double((long long)(lo | hi << 32));
+}
+
+// v^-1/2 to an ulp or two: the instruction's estimate and two steps of Newton's.
+__device__ __forceinline__ double inverse_root(double v) {
+  double y = __builtin_amdgcn_rsq(v);
+#pragma unroll
+  for (int i = 0; i < 2; i++) y = fma(y * 0.5, fma(-(v * y), y, 1.0), y);
+  return y;
 }
 
 // Dims of pair i < D / 2 of a head: (i, i + rot / 2) for the rotated ones, the
@@ -77,75 +113,122 @@ __device__ __forceinline__ void pair_dims(uint32_t i, uint32_t D, uint32_t rot, 
 
 // ---------------------------------------------------------------------------
 // Append.  A workgroup takes 16 token places of a sequence (one block) and one
-// key head, one value head or KV8_Q_HEADS query heads.  A code is decided next
-// to a rounding border, so keys and values are computed in 64 bits (the rate of
-// f64 is far from bounding this: the rows' bytes do), and the codes do not
-// depend on the order of any 32-bit sum.  Angles in 64 bits too, for positions
-// far out: one sine and cosine per pair and half block, the rows between by
-// rotating on.
+// key head, one value head or KV8_Q_HEADS query heads, one a wave.  A code is
+// decided next to a rounding border, so keys and values are computed in 64 bits
+// (the rate of f64 is far from bounding this: the rows' bytes do), and the codes do
+// not depend on the order of any 32-bit sum.  Angles in 64 bits too, for positions
+// far out: two sines and cosines per pair and a run of rows, the rows between by
+// rotating on.  What a workgroup waits for is on its way before it computes the
+// angles: the whole of its rows, and the codes already there.
 // ---------------------------------------------------------------------------
 struct Angle {
   double c, s;
 };
 
+// Half turns a token of pair i: theta^(-2 i / rot) / pi to an ulp or two, 2^x with x =
+// i * (-2 log2(theta) / rot) as the sum of two.
+__device__ __forceinline__ double half_turns(uint32_t i, const Kv8AppendArgs& a) {
+  const double x = (double)i * a.log_hi, x_lo = fma((double)i, a.log_hi, -x) + (double)i * a.log_lo;
+  const double f = exp2(x) * 0.3183098861837907;
+  return fma(f, x_lo * 0.6931471805599453, f);
+}
+
+// The angle of g half turns a token at position pos (the whole turns go first, without
+// a rounding).
+__device__ __forceinline__ Angle angle(double pos, double g) {
+  const double t = pos * g, lo = fma(pos, g, -t);
+  Angle r;
+  sincospi((t - 2.0 * rint(t * 0.5)) + lo, &r.s, &r.c);
+  return r;
+}
+
 // ang[row][pair] for rows [0, nr) at positions pos0 + row.
-__device__ void block_angles(Angle* ang, uint64_t pos0, uint32_t nr, uint32_t rot, float theta) {
-  const uint32_t half = rot / 2;
+__device__ __forceinline__ void block_angles(Angle* ang, uint64_t pos0, uint32_t nr, const Kv8AppendArgs& a) {
+  const uint32_t half = a.rot / 2;
   if (half == 0) return;
   const uint32_t teams = nr > 1 && 256u / half > 1 ? min(256u / half, nr) : 1u;
   const uint32_t per = (nr + teams - 1) / teams;
   for (uint32_t t = threadIdx.x; t < half * teams; t += 256) {
     const uint32_t i = t % half, r0 = (t / half) * per, r1 = min(r0 + per, nr);
     if (r0 >= r1) continue;
-    const double f = pow((double)theta, -2.0 * (double)i / (double)rot);
-    Angle a, st{1.0, 0.0};
-    sincos((double)(pos0 + r0) * f, &a.s, &a.c);
-    if (r1 - r0 > 1) sincos(f, &st.s, &st.c);
+    const double f = half_turns(i, a);
+    Angle g = angle((double)(pos0 + r0), f), st{1.0, 0.0};
+    if (r1 - r0 > 1) st = angle(1.0, f);
     for (uint32_t r = r0; r < r1; r++) {
-      ang[r * half + i] = a;
-      a = Angle{a.c * st.c - a.s * st.s, a.c * st.s + a.s * st.c};
+      ang[r * half + i] = g;
+      g = Angle{g.c * st.c - g.s * st.s, g.c * st.s + g.s * st.c};
     }
   }
 }
 
+// A row's elements of a lane's pairs: loads, and their dims.
 template <int NP>
-__device__ void append_q(const Kv8AppendArgs& a, const Angle* ang, uint32_t row0, uint32_t nr, uint32_t group) {
-  const uint32_t lane = threadIdx.x & 63, wave = wave_id();
-  const uint32_t D = a.c.D, half = a.rot / 2;
-  const uint32_t h0 = group * KV8_Q_HEADS, nh = min(KV8_Q_HEADS, a.nq - h0);
-  for (uint32_t t = wave; t < nr * nh; t += 4) {
-    const uint32_t r = t / nh, h = h0 + t % nh;
-    const float* in = a.q + (uint64_t)(row0 + r) * a.qs + (uint64_t)h * D;
-    float* out = a.qo + (uint64_t)(row0 + r) * a.nq * D + (uint64_t)h * D;
-    float x0[NP], x1[NP], ss = 0.f;
+__device__ __forceinline__ void load_pairs(const float* in, uint32_t D, uint32_t rot, float (&x0)[NP], float (&x1)[NP]) {
 #pragma unroll
-    for (int m = 0; m < NP; m++) {
-      const uint32_t i = lane + 64 * m;
-      x0[m] = x1[m] = 0.f;
-      if (i < D / 2) {
+  for (int m = 0; m < NP; m++) {
+    const uint32_t i = (threadIdx.x & 63) + 64 * m;
+    x0[m] = x1[m] = 0.f;
+    if (i < D / 2) {
+      uint32_t d0, d1;
+      pair_dims(i, D, rot, &d0, &d1);
+      x0[m] = in[d0];
+      x1[m] = in[d1];
+    }
+  }
+}
+
+// Query heads: a wave a head, a few of its rows of the block at a time.
+template <int NP>
+__device__ __forceinline__ void append_q(const Kv8AppendArgs& a, Angle* ang, uint64_t pos0, uint32_t row0, uint32_t nr,
+                                         uint32_t group) {
+  constexpr int R = NP == 4 ? 4 : 8;
+  const uint32_t lane = threadIdx.x & 63, h = group * KV8_Q_HEADS + wave_id();
+  const uint32_t D = a.c.D, half = a.rot / 2;
+  const bool mine = h < a.nq;
+  const float* in = a.q + (uint64_t)row0 * a.qs + (uint64_t)h * D;
+  float* out = a.qo + (uint64_t)row0 * a.nq * D + (uint64_t)h * D;
+  float x0[R][NP], x1[R][NP];
+  const auto load = [&](uint32_t first) {
+#pragma unroll
+    for (int j = 0; j < R; j++)
+      if (mine && first + j < nr) load_pairs<NP>(in + (uint64_t)(first + j) * a.qs, D, a.rot, x0[j], x1[j]);
+  };
+  load(0);
+  block_angles(ang, pos0, nr, a);
+  __syncthreads();
+  for (uint32_t first = 0; first < nr; first += R) {
+    float ss[R];
+#pragma unroll
+    for (int j = 0; j < R; j++) {
+      ss[j] = 0.f;
+      if (!mine || first + j >= nr) continue;
+#pragma unroll
+      for (int m = 0; m < NP; m++) ss[j] += x0[j][m] * x0[j][m] + x1[j][m] * x1[j][m];
+    }
+    const float root = 1.0f / sqrtf(wave_sums<R>(ss) / (float)D + a.eps);  // of row first + lane mod R
+#pragma unroll
+    for (int j = 0; j < R; j++) {
+      const uint32_t r = first + j;
+      if (!mine || r >= nr) continue;
+      __builtin_amdgcn_sched_barrier(0);  // (a row's angles and norms at a time in registers)
+      const float inv = lane_value(root, j);
+#pragma unroll
+      for (int m = 0; m < NP; m++) {
+        const uint32_t i = lane + 64 * m;
+        if (i >= D / 2) continue;
         uint32_t d0, d1;
         pair_dims(i, D, a.rot, &d0, &d1);
-        x0[m] = in[d0];
-        x1[m] = in[d1];
+        const float u = x0[j][m] * inv * a.qn[d0], w = x1[j][m] * inv * a.qn[d1];
+        float c = 1.f, s = 0.f;
+        if (i < half) {
+          c = (float)ang[r * half + i].c;
+          s = (float)ang[r * half + i].s;
+        }
+        out[(uint64_t)r * a.nq * D + d0] = u * c - w * s;
+        out[(uint64_t)r * a.nq * D + d1] = u * s + w * c;
       }
-      ss += x0[m] * x0[m] + x1[m] * x1[m];
     }
-    const float inv = 1.0f / sqrtf(wave_sum(ss) / (float)D + a.eps);
-#pragma unroll
-    for (int m = 0; m < NP; m++) {
-      const uint32_t i = lane + 64 * m;
-      if (i >= D / 2) continue;
-      uint32_t d0, d1;
-      pair_dims(i, D, a.rot, &d0, &d1);
-      const float u = x0[m] * inv * a.qn[d0], w = x1[m] * inv * a.qn[d1];
-      float c = 1.f, s = 0.f;
-      if (i < half) {
-        c = (float)ang[r * half + i].c;
-        s = (float)ang[r * half + i].s;
-      }
-      out[d0] = u * c - w * s;
-      out[d1] = u * s + w * c;
-    }
+    load(first + R);
   }
 }
 
@@ -154,41 +237,50 @@ __device__ __forceinline__ uint32_t k_place(uint32_t t, uint32_t d) { return (d 
 __device__ __forceinline__ uint32_t v_place(uint32_t t, uint32_t d, uint32_t D) { return (t >> 2) * 4 * D + d * 4 + (t & 3); }
 
 template <int NP, bool IS_K>
-__device__ void append_kv(const Kv8AppendArgs& a, const Angle* ang, int8_t* tile, double* red, uint32_t row0,
-                          uint32_t o0, uint32_t nr, uint32_t head, uint32_t at) {
+__device__ __forceinline__ void append_kv(const Kv8AppendArgs& a, Angle* ang, int8_t* tile, double* red, uint64_t pos0,
+                                          uint32_t row0, uint32_t o0, uint32_t nr, uint32_t head, uint32_t at) {
   const uint32_t lane = threadIdx.x & 63, wave = wave_id();
   const uint32_t D = a.c.D, half = a.rot / 2, o1 = o0 + nr;
   int8_t* codes = (IS_K ? a.c.k : a.c.v) + (uint64_t)at * (KV8_BLOCK * D);
   float* scale = (IS_K ? a.c.ks : a.c.vs) + at;
-  const float* src = IS_K || a.k_eq_v ? a.k : a.v;
+  const float* src = (IS_K || a.k_eq_v ? a.k : a.v) + (uint64_t)head * D;
+  // wave w: token places 4 w .. 4 w + 3 of the block
+  float f0[4][NP], f1[4][NP];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const uint32_t t = wave * 4 + j;
+    if (t >= o0 && t < o1) load_pairs<NP>(src + (uint64_t)(row0 + t - o0) * a.kvs, D, a.rot, f0[j], f1[j]);
+  }
   const float old = o0 > 0 ? *scale : 0.f;
   // the codes already there (a fresh block's places without a token become 0)
   int4* t4 = reinterpret_cast<int4*>(tile);
   for (uint32_t i = threadIdx.x; i < D; i += 256) t4[i] = o0 > 0 ? reinterpret_cast<const int4*>(codes)[i] : int4{0, 0, 0, 0};
+  if (IS_K) {
+    block_angles(ang, pos0, nr, a);
+    __syncthreads();
+  }
 
-  // wave w: token places 4 w .. 4 w + 3 of the block
-  double x0[4][NP], x1[4][NP], amax = 0.0;
+  double x0[4][NP], x1[4][NP], ss[4], amax = 0.0;
   bool bad = false;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
     const uint32_t t = wave * 4 + j;
-    const bool mine = t >= o0 && t < o1;
-    const float* in = src + (uint64_t)(row0 + (mine ? t - o0 : 0)) * a.kvs + (uint64_t)head * D;
-    double ss = 0.0;
+    ss[j] = 0.0;
+    if (t < o0 || t >= o1) continue;
 #pragma unroll
     for (int m = 0; m < NP; m++) {
-      const uint32_t i = lane + 64 * m;
-      x0[j][m] = x1[j][m] = 0.0;
-      if (mine && i < D / 2) {
-        uint32_t d0, d1;
-        pair_dims(i, D, a.rot, &d0, &d1);
-        x0[j][m] = (double)in[d0];
-        x1[j][m] = (double)in[d1];
-      }
-      ss += x0[j][m] * x0[j][m] + x1[j][m] * x1[j][m];
+      x0[j][m] = (double)f0[j][m];
+      x1[j][m] = (double)f1[j][m];
+      ss[j] += x0[j][m] * x0[j][m] + x1[j][m] * x1[j][m];
     }
-    if (!mine) continue;
-    const double inv = 1.0 / sqrt(wave_sum(ss) / (double)D + (double)a.eps);
+  }
+  const double root = inverse_root(wave_sums<4>(ss) / (double)D + (double)a.eps);  // of place 4 wave + lane mod 4
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const uint32_t t = wave * 4 + j;
+    if (t < o0 || t >= o1) continue;
+    __builtin_amdgcn_sched_barrier(0);  // (as above)
+    const double inv = lane_value(root, j);
 #pragma unroll
     for (int m = 0; m < NP; m++) {
       const uint32_t i = lane + 64 * m;
@@ -208,7 +300,8 @@ __device__ void append_kv(const Kv8AppendArgs& a, const Angle* ang, int8_t* tile
       }
       x0[j][m] = u;
       x1[j][m] = w;
-      amax = fmax(amax, fmax(fabs(u), fabs(w)));
+      amax = fabs(u) > amax ? fabs(u) : amax;
+      amax = fabs(w) > amax ? fabs(w) : amax;
       bad |= !(fabs(u) < 1e300) || !(fabs(w) < 1e300);
     }
   }
@@ -245,9 +338,9 @@ __device__ void append_kv(const Kv8AppendArgs& a, const Angle* ang, int8_t* tile
       if (i >= D / 2) continue;
       uint32_t d0, d1;
       pair_dims(i, D, a.rot, &d0, &d1);
-      const int c0 = (int)rint(x0[j][m] * inv), c1 = (int)rint(x1[j][m] * inv);
-      tile[IS_K ? k_place(t, d0) : v_place(t, d0, D)] = (int8_t)min(127, max(-127, c0));
-      tile[IS_K ? k_place(t, d1) : v_place(t, d1, D)] = (int8_t)min(127, max(-127, c1));
+      // (at most 127 in magnitude; a NaN becomes 0)
+      tile[IS_K ? k_place(t, d0) : v_place(t, d0, D)] = (int8_t)(int)rint(x0[j][m] * inv);
+      tile[IS_K ? k_place(t, d1) : v_place(t, d1, D)] = (int8_t)(int)rint(x1[j][m] * inv);
     }
   }
   __syncthreads();
@@ -281,16 +374,12 @@ __device__ __forceinline__ void append(const Kv8AppendArgs& a) {
     const uint32_t at = block_at(a.c, page, head, blk);
     const uint32_t o0 = (uint32_t)(p0 - blk * KV8_BLOCK);
     if (unit & 1) {
-      append_kv<NP, false>(a, ang, tile, red, row0, o0, nr, head, at);
+      append_kv<NP, false>(a, ang, tile, red, p0, row0, o0, nr, head, at);
     } else {
-      block_angles(ang, p0, nr, a.rot, a.theta);
-      __syncthreads();
-      append_kv<NP, true>(a, ang, tile, red, row0, o0, nr, head, at);
+      append_kv<NP, true>(a, ang, tile, red, p0, row0, o0, nr, head, at);
     }
   } else {
-    block_angles(ang, p0, nr, a.rot, a.theta);
-    __syncthreads();
-    append_q<NP>(a, ang, row0, nr, unit - 2 * nkv);
+    append_q<NP>(a, ang, p0, row0, nr, unit - 2 * nkv);
   }
 }
 
@@ -1087,6 +1176,18 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, 
   }
 }
 
+namespace {
+// (wide: 16-byte aligned)
+__device__ __forceinline__ void write4(float* to, f32x4 x, uint32_t wide) {
+  if (wide) {
+    *reinterpret_cast<f32x4*>(to) = x;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) to[i] = x[i];
+  }
+}
+}  // namespace
+
 // Read-back: the rows that a batch names as the values their codes stand for;
 // rows of places without a page are 0.  grid (kv heads, blocks, sequences)
 extern "C" __global__ __launch_bounds__(256) void gh_kv8_read_k(Kv8ReadArgs a) {
@@ -1101,34 +1202,34 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_read_k(Kv8ReadArgs a) {
   const uint32_t page = page_of(a.c, a.b, seq, blk);
   const bool has = page < a.c.num_pages;
   const uint32_t at = block_at(a.c, has ? page : 0, head, blk);
-  union Piece {
-    int4 w;
-    int8_t b[16];
-  };
-  for (uint32_t i = threadIdx.x; i < 2 * D; i += 256) {
-    const bool is_k = i < D;
-    float* out = is_k ? a.k : a.v;
-    if (!out) continue;
-    const uint32_t j = is_k ? i : i - D;
-    Piece p;
-    p.w = int4{0, 0, 0, 0};
-    if (has) p.w = reinterpret_cast<const int4*>((is_k ? a.c.k : a.c.v) + (uint64_t)at * (KV8_BLOCK * D))[j];
-    const float s = has ? (is_k ? a.c.ks : a.c.vs)[at] : 0.f;
-    if (is_k) {
-      const uint32_t t = j & 15, d = (j >> 4) * 16;
+  const uint64_t bytes = (uint64_t)at * (KV8_BLOCK * D);
+  // four dims of a token (K), of four tokens (V): a wave's rows of float4 in a row
+  if (a.k) {
+    const float s = has ? a.c.ks[at] : 0.f;
+    for (uint32_t i = threadIdx.x; i < 4 * D; i += 256) {
+      const uint32_t t = i / (D / 4), d = (i % (D / 4)) * 4;
       if (t < o0 || t >= o1) continue;
-      float* to = out + (row0 + t - o0) * kv + (uint64_t)head * D + d;
-#pragma unroll
-      for (int e = 0; e < 16; e++) to[e] = (float)p.b[e] * s;
-    } else {
-      const uint32_t grp = j / (D / 4), d = (j % (D / 4)) * 4;
+      char4 c{0, 0, 0, 0};
+      if (has) c = *reinterpret_cast<const char4*>(a.c.k + bytes + k_place(t, d));
+      write4(a.k + (row0 + t - o0) * kv + (uint64_t)head * D + d, f32x4{(float)c.x, (float)c.y, (float)c.z, (float)c.w} * s, a.wide);
+    }
+  }
+  if (a.v) {
+    const float s = has ? a.c.vs[at] : 0.f;
+    for (uint32_t i = threadIdx.x; i < D; i += 256) {
+      const uint32_t grp = i / (D / 4), d = (i % (D / 4)) * 4;
+      union {
+        int4 w;
+        int8_t b[16];
+      } p;
+      p.w = int4{0, 0, 0, 0};
+      if (has) p.w = reinterpret_cast<const int4*>(a.c.v + bytes)[i];
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const uint32_t t = grp * 4 + e;
         if (t < o0 || t >= o1) continue;
-        float* to = out + (row0 + t - o0) * kv + (uint64_t)head * D + d;
-#pragma unroll
-        for (int r = 0; r < 4; r++) to[r] = (float)p.b[4 * r + e] * s;
+        write4(a.v + (row0 + t - o0) * kv + (uint64_t)head * D + d,
+               f32x4{(float)p.b[e], (float)p.b[4 + e], (float)p.b[8 + e], (float)p.b[12 + e]} * s, a.wide);
       }
     }
   }

@@ -176,8 +176,10 @@ gh_status gh_kv8_append(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8
     a.nq = num_q;
     a.rot = rotary_dim;
     a.k_eq_v = k_eq_v ? 1 : 0;
-    a.theta = theta;
     a.eps = eps;
+    const long double log = rotary_dim ? -2 * log2l((long double)theta) / rotary_dim : 0;
+    a.log_hi = (double)log;
+    a.log_lo = (double)(log - a.log_hi);
     const uint32_t rows = std::min(a.b.max_rows, KV8_BLOCK);
     const unsigned lds = 32 + KV8_BLOCK * a.c.D + rows * (rotary_dim / 2) * 16;
     const dim3 grid(2 * a.c.nkv + (num_q + KV8_Q_HEADS - 1) / KV8_Q_HEADS, touched(a.b), a.b.num_seqs);
@@ -201,6 +203,7 @@ gh_status gh_kv8_read(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8_b
     if (empty(a.b)) return GH_OK;
     a.k = K_out;
     a.v = V_out;
+    a.wide = aligned(K_out, 16) && aligned(V_out, 16);
     void* args[] = {&a};
     return launch(ctx, "gh_kv8_read_k", dim3(a.c.nkv, touched(a.b), a.b.num_seqs), dim3(256), 0, args);
   });
