@@ -3,7 +3,10 @@
 #pragma once
 #include <stdint.h>
 
-#define SAMPLE_CHUNK 4096u  // elements of a row that one workgroup takes
+// Elements of a row that one workgroup of 256 threads takes: 16 a thread, or 4
+// where that leaves CUs idle.
+#define SAMPLE_MANY 16u
+#define SAMPLE_FEW 4u
 
 struct ProbsArgs {
   const float* logits;
@@ -11,7 +14,7 @@ struct ProbsArgs {
   float* part;  // [row][chunk] {max, sum}
   uint64_t stride;
   uint32_t vocab, chunks;
-  float cap, mul;  // soft-cap (0: none); log2(e) / temperature
+  float cap, inv_cap, mul;  // soft-cap (0: none); log2(e) / temperature
 };
 
 struct VerifyArgs {

@@ -2,9 +2,9 @@
 // tokens against them, for gfx950.
 //
 // Both read rows of a vocabulary once or twice and compute little: what bounds
-// them is memory for a batch and latency for one row.  A row is cut into chunks
-// of SAMPLE_CHUNK elements, a workgroup each, so that one row of 262144 spreads
-// over 64 CUs; a second launch joins the chunks.
+// them is memory for a batch and latency for one row.  A row is cut into chunks of
+// 256 N elements, a workgroup each, N = 16, or 4 so that one row of 262144 spreads
+// over every CU; a second launch joins the chunks.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -12,20 +12,18 @@
 
 namespace {
 
-constexpr uint32_t kEach = SAMPLE_CHUNK / 256;  // elements of a thread
-
-// A thread's elements of chunk c: VEC: four float4, 1 KB apart in a wave's row;
-// else single floats.  Elements past the row are `none`.
+// A thread's elements of chunk c: VEC: float4, 1 KB apart in a wave's row; else
+// single floats.  Elements past the row are `none`.
 template <bool VEC>
 __device__ __forceinline__ uint32_t elem(uint32_t i) {
   return VEC ? (i >> 2) * 1024 + threadIdx.x * 4 + (i & 3) : i * 256 + threadIdx.x;
 }
-template <bool VEC>
-__device__ __forceinline__ void load_chunk(const float* row, uint32_t c, uint32_t vocab, float none, float (&x)[kEach]) {
-  const uint32_t base = c * SAMPLE_CHUNK, left = vocab - base;
+template <bool VEC, uint32_t N>
+__device__ __forceinline__ void load_chunk(const float* row, uint32_t c, uint32_t vocab, float none, float (&x)[N]) {
+  const uint32_t base = c * (256 * N), left = vocab - base;
   row += base;
 #pragma unroll
-  for (uint32_t i = 0; i < kEach; i += VEC ? 4 : 1) {
+  for (uint32_t i = 0; i < N; i += VEC ? 4 : 1) {
     const uint32_t e = elem<VEC>(i);
     if (VEC) {  // (vocab is a multiple of 4 there)
       float4 v = {none, none, none, none};
@@ -46,8 +44,42 @@ __device__ __forceinline__ void load_chunk(const float* row, uint32_t c, uint32_
 // maximum and sum, the second joins a row's and writes; it finds the logits in
 // the last-level cache.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ float capped(float x, float cap) {
-  return cap > 0.f && x != -INFINITY ? cap * tanhf(x / cap) : x;
+// tanh within 5 half steps, without the library's branches, which bounded the
+// kernels (40 rows of 262144: 17 us a launch at 2.5 TB/s): below 0.7 y + y^3 P(y^2),
+// P fitted by least squares at Chebyshev nodes (relative error 8e-10 before
+// rounding), above 1 - 2 / (e^2y + 1).
+__device__ __forceinline__ float tanh_low(float y) {
+  const float t = y * y;
+  float p = 0.00188978482f;
+  p = fmaf(p, t, -0.00787458383f);
+  p = fmaf(p, t, 0.0215662047f);
+  p = fmaf(p, t, -0.0539197139f);
+  p = fmaf(p, t, 0.13332969f);
+  p = fmaf(p, t, -0.333333254f);
+  return fmaf(y * t, p, y);
+}
+__device__ __forceinline__ float tanh_high(float y) {
+  const float e = __builtin_amdgcn_exp2f(fabsf(y) * 2.885390082f);
+  return copysignf(fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f), y);
+}
+// A thread's logits soft-capped.  Most rows have nothing past 0.7 cap: a wave
+// without takes the first form alone.
+template <uint32_t N>
+__device__ __forceinline__ void soft_cap(float (&x)[N], float cap, float inv_cap) {
+  if (!(cap > 0.f)) return;
+  bool far = false;
+#pragma unroll
+  for (uint32_t i = 0; i < N; i++) far |= !(fabsf(x[i] * inv_cap) < 0.7f);
+  if (__any(far)) {
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) {
+      const float y = x[i] * inv_cap;
+      if (x[i] != -INFINITY) x[i] = cap * (fabsf(y) < 0.7f ? tanh_low(y) : tanh_high(y));
+    }
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) x[i] = cap * tanh_low(x[i] * inv_cap);
+  }
 }
 
 // the workgroup's maximum and the sum relative to it, in every thread
@@ -59,7 +91,7 @@ __device__ __forceinline__ void join(float* m, float* l, float mul) {
     const float m2 = __shfl_xor(M, off, 64), l2 = __shfl_xor(L, off, 64), mx = fmaxf(M, m2);
     const float base = mx == -INFINITY ? 0.f : mx;
     // in the order of the lanes, so that both of a pair get the same sum
-    const float a = L * exp2f((M - base) * mul), b = l2 * exp2f((m2 - base) * mul);
+    const float a = L * __builtin_amdgcn_exp2f((M - base) * mul), b = l2 * __builtin_amdgcn_exp2f((m2 - base) * mul);
     L = a + b;
     M = mx;
   }
@@ -73,24 +105,22 @@ __device__ __forceinline__ void join(float* m, float* l, float mul) {
   const float base = M == -INFINITY ? 0.f : M;
   L = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; w++) L += sl[w] * exp2f((sm[w] - base) * mul);
+  for (int w = 0; w < 4; w++) L += sl[w] * __builtin_amdgcn_exp2f((sm[w] - base) * mul);
   *m = M;
   *l = L;
 }
 
 // grid (chunks, rows)
-template <bool VEC>
+template <bool VEC, uint32_t N>
 __device__ __forceinline__ void probs_part(const ProbsArgs& a) {
-  float x[kEach], m = -INFINITY, l = 0.f;
-  load_chunk<VEC>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
+  float x[N], m = -INFINITY, l = 0.f;
+  load_chunk<VEC, N>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
+  soft_cap<N>(x, a.cap, a.inv_cap);
 #pragma unroll
-  for (uint32_t i = 0; i < kEach; i++) {
-    x[i] = capped(x[i], a.cap);
-    m = fmaxf(m, x[i]);
-  }
+  for (uint32_t i = 0; i < N; i++) m = fmaxf(m, x[i]);
   const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-  for (uint32_t i = 0; i < kEach; i++) l += exp2f((x[i] - base) * a.mul);
+  for (uint32_t i = 0; i < N; i++) l += __builtin_amdgcn_exp2f((x[i] - base) * a.mul);
   join(&m, &l, a.mul);
   if (threadIdx.x == 0) {
     float* p = a.part + 2 * ((uint64_t)blockIdx.y * a.chunks + blockIdx.x);
@@ -99,25 +129,26 @@ __device__ __forceinline__ void probs_part(const ProbsArgs& a) {
   }
 }
 
-template <bool VEC>
+template <bool VEC, uint32_t N>
 __device__ __forceinline__ void probs_write(const ProbsArgs& a) {
-  float x[kEach], m = -INFINITY, l = 0.f;
-  load_chunk<VEC>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
+  float x[N], m = -INFINITY, l = 0.f;
+  load_chunk<VEC, N>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
   const float* p = a.part + 2 * (uint64_t)blockIdx.y * a.chunks;
   for (uint32_t c = threadIdx.x; c < a.chunks; c += 256) {
     const float m2 = p[2 * c], l2 = p[2 * c + 1], mx = fmaxf(m, m2), base = mx == -INFINITY ? 0.f : mx;
-    l = l * exp2f((m - base) * a.mul) + l2 * exp2f((m2 - base) * a.mul);
+    l = l * __builtin_amdgcn_exp2f((m - base) * a.mul) + l2 * __builtin_amdgcn_exp2f((m2 - base) * a.mul);
     m = mx;
   }
+  soft_cap<N>(x, a.cap, a.inv_cap);
   join(&m, &l, a.mul);
   const float base = m == -INFINITY ? 0.f : m;
   const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;  // every logit -inf: all 0
-  const uint32_t start = blockIdx.x * SAMPLE_CHUNK, left = a.vocab - start;
+  const uint32_t start = blockIdx.x * (256 * N), left = a.vocab - start;
   float* out = a.probs + blockIdx.y * a.stride + start;
 #pragma unroll
-  for (uint32_t i = 0; i < kEach; i++) x[i] = exp2f((capped(x[i], a.cap) - base) * a.mul) * inv;
+  for (uint32_t i = 0; i < N; i++) x[i] = __builtin_amdgcn_exp2f((x[i] - base) * a.mul) * inv;
 #pragma unroll
-  for (uint32_t i = 0; i < kEach; i += VEC ? 4 : 1) {
+  for (uint32_t i = 0; i < N; i += VEC ? 4 : 1) {
     const uint32_t e = elem<VEC>(i);
     if (e >= left) continue;
     if (VEC) {
@@ -138,35 +169,30 @@ struct Stop {
   uint32_t kept, drafts;
 };
 
-// how many drafts of sequence b are kept (every workgroup finds it for itself:
-// a few scattered loads)
+// how many drafts of sequence b are kept (every wave finds it for itself: a few
+// scattered loads)
 __device__ __forceinline__ Stop stop_of(const VerifyArgs& a, uint32_t b) {
-  __shared__ uint32_t s;
-  const uint32_t n = a.n_draft ? min(a.n_draft[b], a.max_draft) : a.max_draft;
-  if (threadIdx.x < 64) {
-    uint32_t kept = n;
-    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
-      const uint32_t i = i0 + threadIdx.x;
-      bool fine = true;
-      if (i < n) {
-        const uint32_t x = a.tokens[(uint64_t)b * a.max_draft + i];
-        fine = false;
-        if (x < a.vocab) {
-          const double p = a.target[((uint64_t)b * (a.max_draft + 1) + i) * a.vocab + x];
-          const double q = a.draft ? (double)a.draft[((uint64_t)b * a.max_draft + i) * a.vocab + x] : 1.0;
-          fine = (double)a.u[(uint64_t)b * a.max_draft + i] * q < p;
-        }
-      }
-      const uint64_t bad = __ballot(!fine);
-      if (bad) {
-        kept = i0 + (uint32_t)__builtin_ctzll(bad);
-        break;
+  const uint32_t n = a.n_draft ? min(a.n_draft[b], a.max_draft) : a.max_draft, lane = threadIdx.x & 63;
+  uint32_t kept = n;
+  for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+    const uint32_t i = i0 + lane;
+    bool fine = true;
+    if (i < n) {
+      const uint32_t x = a.tokens[(uint64_t)b * a.max_draft + i];
+      fine = false;
+      if (x < a.vocab) {
+        const double p = a.target[((uint64_t)b * (a.max_draft + 1) + i) * a.vocab + x];
+        const double q = a.draft ? (double)a.draft[((uint64_t)b * a.max_draft + i) * a.vocab + x] : 1.0;
+        fine = (double)a.u[(uint64_t)b * a.max_draft + i] * q < p;
       }
     }
-    if (threadIdx.x == 0) s = kept;
+    const uint64_t bad = __ballot(!fine);
+    if (bad) {
+      kept = i0 + (uint32_t)__builtin_ctzll(bad);
+      break;
+    }
   }
-  __syncthreads();
-  return Stop{s, n};
+  return Stop{(uint32_t)__builtin_amdgcn_readfirstlane(kept), n};
 }
 
 // weight of element v where sequence b stops: left over the draft, and the target's
@@ -196,22 +222,23 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 
 // grid (chunks, sequences)
-template <bool VEC>
+template <bool VEC, uint32_t N>
 __device__ __forceinline__ void verify_part(const VerifyArgs& a) {
   const uint32_t b = blockIdx.y, c = blockIdx.x;
-  const Rows r = rows_of(a, b, stop_of(a, b));
-  float p[kEach], q[kEach];
-  load_chunk<VEC>(r.p, c, a.vocab, 0.f, p);
+  const Stop s = stop_of(a, b);
+  const Rows r = rows_of(a, b, s);
+  float p[N], q[N];
+  load_chunk<VEC, N>(r.p, c, a.vocab, 0.f, p);
   if (r.q) {
-    load_chunk<VEC>(r.q, c, a.vocab, 0.f, q);
+    load_chunk<VEC, N>(r.q, c, a.vocab, 0.f, q);
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; i++) q[i] = 0.f;
+    for (uint32_t i = 0; i < N; i++) q[i] = 0.f;
   }
   double w = 0.0, t = 0.0;
 #pragma unroll
-  for (uint32_t i = 0; i < kEach; i++) {
-    w += over(p[i], q[i], c * SAMPLE_CHUNK + elem<VEC>(i) == r.cut);
+  for (uint32_t i = 0; i < N; i++) {
+    w += over(p[i], q[i], c * (256 * N) + elem<VEC>(i) == r.cut);
     t += plain(p[i]);
   }
   w = wave_sum(w);
@@ -226,123 +253,136 @@ __device__ __forceinline__ void verify_part(const VerifyArgs& a) {
     double* out = a.part + 2 * ((uint64_t)b * a.chunks + c);
     out[0] = sw[0] + sw[1] + (sw[2] + sw[3]);
     out[1] = st[0] + st[1] + (st[2] + st[3]);
+    if (c == 0) a.accepted[b] = s.kept;
   }
 }
 
-// Inclusive sums over the workgroup's threads, in their order.
-__device__ __forceinline__ double scan(double v, double* total) {
-  __shared__ double s[4];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Inclusive sums over the wave's lanes.
+__device__ __forceinline__ double wave_scan(double v) {
+  const uint32_t lane = threadIdx.x & 63;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const double u = __shfl_up(v, off, 64);
     if (lane >= (uint32_t)off) v += u;
   }
-  __syncthreads();
-  if (lane == 63) s[wave] = v;
-  __syncthreads();
-  double before = 0.0;
-  for (uint32_t w = 0; w < wave; w++) before += s[w];
-  *total = s[0] + s[1] + s[2] + s[3];
-  return before + v;
+  return v;
 }
 
-// The least index whose mark is set, 0xffffffff if there is none; `last`: the greatest.
-__device__ __forceinline__ uint32_t pick_index(bool mark, uint32_t index, bool last) {
-  __shared__ uint32_t s[4];
-  uint32_t v = mark ? (last ? 0xfffffffeu - index : index) : 0xffffffffu;  // (index below 2^31)
+// N elements of a row from v0 on (0 past its end, or without a row).
+template <bool VEC, uint32_t N>
+__device__ __forceinline__ void row_part(const float* row, uint32_t v0, uint32_t vocab, float (&x)[N]) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = min(v, (uint32_t)__shfl_xor((int)v, off, 64));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = min(min(s[0], s[1]), min(s[2], s[3]));
-  return v == 0xffffffffu ? v : last ? 0xfffffffeu - v : v;
+  for (uint32_t i = 0; i < N; i += VEC ? 4 : 1) {
+    if (VEC) {
+      float4 v = {0.f, 0.f, 0.f, 0.f};
+      if (row && v0 + i < vocab) v = *reinterpret_cast<const float4*>(row + v0 + i);
+      x[i] = v.x;
+      x[i + 1] = v.y;
+      x[i + 2] = v.z;
+      x[i + 3] = v.w;
+    } else {
+      x[i] = row && v0 + i < vocab ? row[v0 + i] : 0.f;
+    }
+  }
 }
 
-}  // namespace
-
-extern "C" __global__ __launch_bounds__(256) void gh_probs_part_v4_k(ProbsArgs a) { probs_part<true>(a); }
-extern "C" __global__ __launch_bounds__(256) void gh_probs_part_v1_k(ProbsArgs a) { probs_part<false>(a); }
-extern "C" __global__ __launch_bounds__(256) void gh_probs_write_v4_k(ProbsArgs a) { probs_write<true>(a); }
-extern "C" __global__ __launch_bounds__(256) void gh_probs_write_v1_k(ProbsArgs a) { probs_write<false>(a); }
-extern "C" __global__ __launch_bounds__(256) void gh_verify_part_v4_k(VerifyArgs a) { verify_part<true>(a); }
-extern "C" __global__ __launch_bounds__(256) void gh_verify_part_v1_k(VerifyArgs a) { verify_part<false>(a); }
-
-// The token of each sequence: the chunk that the drawn share falls into, then the
-// element.  grid (sequences)
-extern "C" __global__ __launch_bounds__(256) void gh_verify_token_k(VerifyArgs a) {
-  const uint32_t b = blockIdx.x, tid = threadIdx.x;
-  const Stop st = stop_of(a, b);
-  const Rows r = rows_of(a, b, st);
+// The token of a sequence: the chunk that the drawn share falls into (every wave
+// finds it for itself, its lanes a run of chunks each), then the element.
+// grid (sequences)
+template <bool VEC, uint32_t N>
+__device__ __forceinline__ void verify_token(const VerifyArgs& a) {
+  const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t kept = a.accepted[b];  // (the first launch's)
+  const uint32_t drafts = a.n_draft ? min(a.n_draft[b], a.max_draft) : a.max_draft;
+  const Rows r = rows_of(a, b, Stop{kept, drafts});
   const double* part = a.part + 2 * (uint64_t)b * a.chunks;
-  // the sums of a thread's run of chunks
-  const uint32_t per = (a.chunks + 255) / 256, c0 = min(tid * per, a.chunks), c1 = min(c0 + per, a.chunks);
+  const uint32_t per = (a.chunks + 63) / 64, c0 = min(lane * per, a.chunks), c1 = min(c0 + per, a.chunks);
   double w = 0.0, t = 0.0;
   for (uint32_t c = c0; c < c1; c++) {
     w += part[2 * c];
     t += part[2 * c + 1];
   }
-  double total_w, total_t;
-  const double cw = scan(w, &total_w), ct = scan(t, &total_t);
+  const double cw = wave_scan(w), ct = wave_scan(t);
+  const double total_w = __shfl(cw, 63, 64), total_t = __shfl(ct, 63, 64);
   const bool left = total_w > 0.0;  // else (the draft covers the target) the target itself
-  const double total = left ? total_w : total_t, mine = left ? w : t;
+  const double total = left ? total_w : total_t, mine = left ? w : t, upto = left ? cw : ct;
   uint32_t token = 0xffffffffu;
   if (total > 0.0 && total < HUGE_VAL) {
     float u = a.pick[b];
     u = u > 0.f ? u : 0.f;
     const double goal = (double)u * total;
-    // the thread whose run of chunks holds it (past the end: the last that weighs)
-    const double upto = left ? cw : ct;
-    uint32_t who = pick_index(upto > goal && mine > 0.0, tid, false);
-    if (who == 0xffffffffu) who = pick_index(mine > 0.0, tid, true);
-    __shared__ double s_before;
-    __shared__ uint32_t s_chunk;
-    if (tid == who) {
-      double before = upto - mine;
-      uint32_t c = c0, last = c0;
-      double last_before = before;
-      for (; c < c1; c++) {
-        const double x = part[2 * c + (left ? 0 : 1)];
-        if (x > 0.0) {
-          last = c;
-          last_before = before;
-          if (before + x > goal) break;
-        }
-        before += x;
+    // the lane whose run of chunks holds it (past the end: the last that weighs)
+    const uint64_t hits = __ballot(upto > goal && mine > 0.0), some = __ballot(mine > 0.0);
+    const int who = hits ? __builtin_ctzll(hits) : 63 - __builtin_clzll(some);
+    double before = __shfl(upto - mine, who, 64), run = before;
+    uint32_t chunk = 0;
+    const uint32_t w0 = min((uint32_t)who * per, a.chunks), w1 = min(w0 + per, a.chunks);
+    for (uint32_t c = w0; c < w1; c++) {
+      const double x = part[2 * c + (left ? 0 : 1)];
+      if (x > 0.0) {
+        chunk = c;
+        before = run;
+        if (run + x > goal) break;
       }
-      s_chunk = last;
-      s_before = last_before;
+      run += x;
     }
-    __syncthreads();
-    const uint32_t c = s_chunk, base = c * SAMPLE_CHUNK, v0 = base + tid * kEach;
-    const double before = s_before;
-    double e[kEach], sum = 0.0, chunk_total;
-    bool any = false;
+    // the chunk's elements, N in a row a thread
+    const uint32_t v0 = chunk * (256 * N) + tid * N;
+    double e[N], sum = 0.0;
+    uint32_t last = 0xffffffffu, hit = 0xffffffffu;
+    float p[N], q[N];
+    row_part<VEC, N>(r.p, v0, a.vocab, p);
+    row_part<VEC, N>(left ? r.q : nullptr, v0, a.vocab, q);
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; i++) {
-      const uint32_t v = v0 + i;
-      e[i] = 0.0;
-      if (v < a.vocab) e[i] = left ? over(r.p[v], r.q ? r.q[v] : 0.f, v == r.cut) : plain(r.p[v]);
-      any |= e[i] > 0.0;
+    for (uint32_t i = 0; i < N; i++) {
+      e[i] = left ? over(p[i], q[i], v0 + i == r.cut) : plain(p[i]);
+      if (e[i] > 0.0) last = v0 + i;
       sum += e[i];
     }
-    double run = before + (scan(sum, &chunk_total) - sum);
-    uint32_t hit = 0xffffffffu, last = 0;
+    __shared__ double waves[4];
+    __shared__ uint32_t found[8];
+    const double upto_here = wave_scan(sum);
+    if (lane == 63) waves[wave] = upto_here;
+    __syncthreads();
+    for (uint32_t k = 0; k < wave; k++) before += waves[k];
+    double here = before + (upto_here - sum);
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; i++) {
-      run += e[i];
-      if (e[i] > 0.0) {
-        last = v0 + i;
-        if (hit == 0xffffffffu && run > goal) hit = v0 + i;
-      }
+    for (uint32_t i = 0; i < N; i++) {
+      here += e[i];
+      if (e[i] > 0.0 && hit == 0xffffffffu && here > goal) hit = v0 + i;
     }
-    token = pick_index(hit != 0xffffffffu, hit, false);
-    if (token == 0xffffffffu) token = pick_index(any, last, true);
+    const uint64_t with_hit = __ballot(hit != 0xffffffffu), with_any = __ballot(last != 0xffffffffu);
+    const uint32_t first_hit = __shfl(hit, with_hit ? __builtin_ctzll(with_hit) : 0, 64);
+    const uint32_t last_any = __shfl(last, with_any ? 63 - __builtin_clzll(with_any) : 0, 64);
+    if (lane == 0) {
+      found[wave] = with_hit ? first_hit : 0xffffffffu;
+      found[4 + wave] = with_any ? last_any : 0xffffffffu;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 3; k >= 0; k--)
+      if (found[k] != 0xffffffffu) token = found[k];
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (token == 0xffffffffu && found[7 - k] != 0xffffffffu) token = found[7 - k];
   }
   const uint32_t width = a.max_draft + 1;
   for (uint32_t i = tid; i < width; i += 256)
     a.out[(uint64_t)b * width + i] =
-        i < st.kept ? a.tokens[(uint64_t)b * a.max_draft + i] : i == st.kept ? token : 0xffffffffu;
-  if (tid == 0) a.accepted[b] = st.kept;
+        i < kept ? a.tokens[(uint64_t)b * a.max_draft + i] : i == kept ? token : 0xffffffffu;
 }
+
+}  // namespace
+
+// N elements a thread, 16-byte loads (v4) or single ones (v1)
+#define SAMPLE(N)                                                                                                     \
+  extern "C" __global__ __launch_bounds__(256) void gh_probs_part_n##N##_v4_k(ProbsArgs a) { probs_part<true, N>(a); }   \
+  extern "C" __global__ __launch_bounds__(256) void gh_probs_part_n##N##_v1_k(ProbsArgs a) { probs_part<false, N>(a); }  \
+  extern "C" __global__ __launch_bounds__(256) void gh_probs_write_n##N##_v4_k(ProbsArgs a) { probs_write<true, N>(a); } \
+  extern "C" __global__ __launch_bounds__(256) void gh_probs_write_n##N##_v1_k(ProbsArgs a) { probs_write<false, N>(a); } \
+  extern "C" __global__ __launch_bounds__(256) void gh_verify_part_n##N##_v4_k(VerifyArgs a) { verify_part<true, N>(a); } \
+  extern "C" __global__ __launch_bounds__(256) void gh_verify_part_n##N##_v1_k(VerifyArgs a) { verify_part<false, N>(a); } \
+  extern "C" __global__ __launch_bounds__(256) void gh_verify_token_n##N##_v4_k(VerifyArgs a) { verify_token<true, N>(a); } \
+  extern "C" __global__ __launch_bounds__(256) void gh_verify_token_n##N##_v1_k(VerifyArgs a) { verify_token<false, N>(a); }
+SAMPLE(4)
+SAMPLE(16)

@@ -122,7 +122,14 @@ gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, co
   return GH_OK;
 }
 
-uint32_t chunks_of(uint32_t vocab) { return (uint32_t)(((uint64_t)vocab + SAMPLE_CHUNK - 1) / SAMPLE_CHUNK); }
+// Elements of a thread in the sampling kernels: 16, or 4 while that gives fewer
+// workgroups than CUs (one row of 262144: probabilities 7.5 us
+// with 4 a thread, 9.9 with 16; verification 8.7 and 10.9).
+uint32_t sample_each(const gh_context* ctx, uint32_t rows, uint32_t vocab) {
+  const uint64_t many = (vocab + 256ull * SAMPLE_MANY - 1) / (256 * SAMPLE_MANY);
+  return rows * many < (uint64_t)ctx->num_cus ? SAMPLE_FEW : SAMPLE_MANY;
+}
+uint32_t chunks_of(uint32_t vocab, uint32_t each) { return (uint32_t)((vocab + 256ull * each - 1) / (256 * each)); }
 
 gh_status check_work(const char* who, const void* work, size_t have, size_t need) {
   if (need == 0) return GH_OK;
@@ -266,8 +273,8 @@ gh_status gh_kv8_attn(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8_b
   });
 }
 
-size_t gh_logit_probs_workspace(const gh_context*, uint32_t rows, uint32_t vocab) {
-  return (size_t)rows * chunks_of(vocab) * 2 * sizeof(float);
+size_t gh_logit_probs_workspace(const gh_context* ctx, uint32_t rows, uint32_t vocab) {
+  return ctx ? (size_t)rows * chunks_of(vocab, sample_each(ctx, rows, vocab)) * 2 * sizeof(float) : 0;
 }
 
 gh_status gh_logit_probs(gh_context* ctx, const float* logits, float* probs, uint32_t rows, uint32_t vocab,
@@ -284,20 +291,23 @@ gh_status gh_logit_probs(gh_context* ctx, const float* logits, float* probs, uin
     if (!aligned(logits, 4) || !aligned(probs, 4)) return invalid(who, "rows must be 4-byte aligned");
     gh_status st = check_work(who, work, work_bytes, gh_logit_probs_workspace(ctx, rows, vocab));
     if (st != GH_OK) return st;
-    ProbsArgs a{logits, probs, static_cast<float*>(work), stride, vocab, chunks_of(vocab), softcap,
-                (float)(1.4426950408889634 / (double)temperature)};
+    const uint32_t each = sample_each(ctx, rows, vocab);
+    ProbsArgs a{logits, probs, static_cast<float*>(work), stride, vocab, chunks_of(vocab, each), softcap,
+                softcap > 0.f ? 1.f / softcap : 0.f, (float)(1.4426950408889634 / (double)temperature)};
     if (!(a.mul < INFINITY)) return invalid(who, "temperature is too small");
+    if (!(a.inv_cap < INFINITY)) return invalid(who, "softcap is too small");
     const bool vec = vocab % 4 == 0 && stride % 4 == 0 && aligned(logits, 16) && aligned(probs, 16);
     void* args[] = {&a};
     const dim3 grid(a.chunks, rows);
-    st = launch(ctx, vec ? "gh_probs_part_v4_k" : "gh_probs_part_v1_k", grid, dim3(256), 0, args);
+    const std::string form = "_n" + std::to_string(each) + (vec ? "_v4_k" : "_v1_k");
+    st = launch(ctx, ("gh_probs_part" + form).c_str(), grid, dim3(256), 0, args);
     if (st != GH_OK) return st;
-    return launch(ctx, vec ? "gh_probs_write_v4_k" : "gh_probs_write_v1_k", grid, dim3(256), 0, args);
+    return launch(ctx, ("gh_probs_write" + form).c_str(), grid, dim3(256), 0, args);
   });
 }
 
-size_t gh_spec_verify_workspace(const gh_context*, uint32_t num_seqs, uint32_t vocab) {
-  return (size_t)num_seqs * chunks_of(vocab) * 2 * sizeof(double);
+size_t gh_spec_verify_workspace(const gh_context* ctx, uint32_t num_seqs, uint32_t vocab) {
+  return ctx ? (size_t)num_seqs * chunks_of(vocab, sample_each(ctx, num_seqs, vocab)) * 2 * sizeof(double) : 0;
 }
 
 gh_status gh_spec_verify(gh_context* ctx, const float* target, const float* draft, const uint32_t* tokens,
@@ -319,13 +329,15 @@ gh_status gh_spec_verify(gh_context* ctx, const float* target, const float* draf
       if (!aligned(p, 4)) return invalid(who, "arrays must be 4-byte aligned");
     gh_status st = check_work(who, work, work_bytes, gh_spec_verify_workspace(ctx, num_seqs, vocab));
     if (st != GH_OK) return st;
+    const uint32_t each = sample_each(ctx, num_seqs, vocab);
     VerifyArgs a{target, draft, tokens, n_draft, u, pick, out_tokens, accepted, static_cast<double*>(work),
-                 max_draft, vocab, chunks_of(vocab)};
+                 max_draft, vocab, chunks_of(vocab, each)};
     const bool vec = vocab % 4 == 0 && aligned(target, 16) && aligned(draft, 16);
     void* args[] = {&a};
-    st = launch(ctx, vec ? "gh_verify_part_v4_k" : "gh_verify_part_v1_k", dim3(a.chunks, num_seqs), dim3(256), 0, args);
+    const std::string form = "_n" + std::to_string(each) + (vec ? "_v4_k" : "_v1_k");
+    st = launch(ctx, ("gh_verify_part" + form).c_str(), dim3(a.chunks, num_seqs), dim3(256), 0, args);
     if (st != GH_OK) return st;
-    return launch(ctx, "gh_verify_token_k", dim3(num_seqs), dim3(256), 0, args);
+    return launch(ctx, ("gh_verify_token" + form).c_str(), dim3(num_seqs), dim3(256), 0, args);
   });
 }
 
