@@ -403,6 +403,7 @@ __device__ __forceinline__ void append(const Kv8AppendArgs& a) {
 // ---------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kNoExp = -100000;
+constexpr int kLazy = 4;  // of the kernel of many columns
 
 __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
   // byte ^ 0x80 under the exponent of 1024 is 1152 + code
@@ -427,8 +428,8 @@ __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
 struct Tile {
   uint32_t seq, head, first, rows, col0, ncol;
   uint64_t past, lo, hi;  // tokens [lo, hi) are visible to one of its columns
-  uint64_t all_lo, all_hi; // tokens [all_lo, all_hi) to every one of them, where there is a page
   uint32_t step0, steps;  // steps of 32 tokens that hold them
+  uint32_t all0, all1;    // steps [all0, all1): every token visible to every column, where there is a page
 };
 
 // false: the tile has no row
@@ -449,8 +450,8 @@ __device__ __forceinline__ bool tile_of(const Kv8AttnArgs& a, uint32_t seq, uint
   const uint64_t hi = min(p1 + 1, held);
   t->lo = lo;
   t->hi = hi;
-  t->all_lo = a.window && p1 + 1 > a.window ? p1 + 1 - a.window : 0;
-  t->all_hi = p0 + 1;
+  t->all0 = a.window && p1 + 1 > a.window ? (uint32_t)((p1 + KV8_STEP - a.window) / KV8_STEP) : 0;
+  t->all1 = (uint32_t)((p0 + 1) / KV8_STEP);
   t->step0 = (uint32_t)(lo / KV8_STEP);
   t->steps = hi > lo ? (uint32_t)((hi + KV8_STEP - 1) / KV8_STEP) - t->step0 : 0u;
   return true;
@@ -544,32 +545,40 @@ __device__ __forceinline__ f16x2 half2(float a, float b) {
   return __builtin_convertvector((f32x2{a, b}), f16x2);
 }
 
+// The scale that a block's scores take: NaN where its values' scale is no number, so
+// that what sees one of them is NaN.  (Uniform; 0 where there is no page.)
+__device__ __forceinline__ bool scale_number(float v) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane(__float_as_uint(v)) < 0x7f800000u;
+}
+
 // The softmax of a step's scores sc, in units of log2 (-inf: not seen): the halves
 // of P for the second product, and the running values.  vs: the blocks' scales of V.
-template <int NL>
+// What is subtracted from the scores follows their maximum when that is over it by
+// more than LAZY, so P is at most 2^LAZY (and its halves are in units that much
+// larger): with 16 columns one or another has a new maximum in most steps of a
+// prompt, and each costs a product for every sum.
+template <int NL, int LAZY>
 __device__ __forceinline__ void soft_step(const float (&sc)[2][4], const float (&vs)[2], const bool (&has)[2], Run<NL>* r,
                                           f16x8* phi, f16x8* plo) {
-  float mx = r->m, vmul[2];
+  float mx = sc[0][0], vmul[2];
   int E = r->E;
-  bool odd = false;  // a scale that is no number
 #pragma unroll
   for (int b = 0; b < 2; b++) {
 #pragma unroll
     for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[b][i]);
     // the exponent of a scale that counts (a power of two; 0 has none)
     const uint32_t bits = __builtin_amdgcn_readfirstlane(__float_as_uint(vs[b]));
-    const bool number = bits - 1u < 0x7f800000u - 1u;
-    odd |= has[b] && bits >= 0x7f800000u;
-    if (has[b] && number) E = max(E, (int)(bits >> 23) - 127);
+    if (has[b] && bits - 1u < 0x7f800000u - 1u) E = max(E, (int)(bits >> 23) - 127);
   }
   mx = column_max(mx);
+  mx = mx > r->m + LAZY ? mx : r->m;
   const float base = mx == -INFINITY ? 0.f : mx;
   const float alpha = __builtin_amdgcn_exp2f(r->m - base);
   const float turn = r->E == E ? alpha : alpha * ldexpf(1.f, max(r->E - E, -200));
   r->m = mx;
   r->E = E;
 #pragma unroll
-  for (int b = 0; b < 2; b++) vmul[b] = has[b] ? ldexpf(vs[b], E == kNoExp ? 0 : 14 - E) : 0.f;
+  for (int b = 0; b < 2; b++) vmul[b] = has[b] && scale_number(vs[b]) ? ldexpf(vs[b], E == kNoExp ? 0 : 14 - LAZY - E) : 0.f;
   if (__any(turn != 1.f)) {
 #pragma unroll
     for (int l = 0; l < NL; l++)
@@ -589,10 +598,6 @@ __device__ __forceinline__ void soft_step(const float (&sc)[2][4], const float (
       const float p = __builtin_amdgcn_exp2f(sc[b][i] - base);
       sum += p;
       w[i] = p * vmul[b];
-    }
-    if (odd) {  // (a NaN score is seen)
-#pragma unroll
-      for (int i = 0; i < 4; i++) w[i] = sc[b][i] != -INFINITY ? w[i] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 2; i++) {
@@ -622,19 +627,19 @@ __device__ __forceinline__ void settle(i32x4 (&acc)[2][4]) {
 
 // Scores, in units of log2, from their digit sums; -inf: not seen.
 __device__ __forceinline__ void finish_scores(const Kv8AttnArgs& a, i32x4 (&acc)[2][4], const float (&ks)[2],
-                                              const bool (&has)[2], float qmul, const Tile& t, int64_t pos, uint32_t step,
-                                              float (&sc)[2][4]) {
+                                              const float (&vs)[2], const bool (&has)[2], float qmul, const Tile& t,
+                                              int64_t pos, uint32_t step, float (&sc)[2][4]) {
   const uint32_t g = (threadIdx.x & 63) >> 4;
   settle(acc);
 #pragma unroll
   for (int b = 0; b < 2; b++) {
-    const float mul = qmul * ks[b];  // (powers of two and the constant: one rounding, of the constant)
+    // (powers of two and the constant: one rounding, of the constant)
+    const float mul = qmul * (scale_number(vs[b]) ? ks[b] : __builtin_nanf(""));
 #pragma unroll
     for (int i = 0; i < 4; i++) sc[b][i] = digit_sum(acc[b][3][i], acc[b][2][i], acc[b][1][i], acc[b][0][i]) * mul;
   }
-  // every token of the step is seen by every column
-  const bool whole = has[0] && has[1] && (uint64_t)step * KV8_STEP >= t.all_lo && ((uint64_t)step + 1) * KV8_STEP <= t.all_hi;
-  if (!whole) {
+  // unless every token of the step is seen by every column
+  if (!has[0] || !has[1] || step < t.all0 || step >= t.all1) {
 #pragma unroll
     for (int b = 0; b < 2; b++) {
       const int64_t t0 = (int64_t)step * KV8_STEP + b * KV8_BLOCK + 4 * g;
@@ -646,8 +651,8 @@ __device__ __forceinline__ void finish_scores(const Kv8AttnArgs& a, i32x4 (&acc)
 
 // Scores of a step's tokens 4 g .. of both blocks for a lane's column.
 template <int NL>
-__device__ __forceinline__ void score_step(const Kv8AttnArgs& a, const Codes<NL>& k, const i32x4* qd, float qmul,
-                                           const Tile& t, int64_t pos, uint32_t step, float (&sc)[2][4]) {
+__device__ __forceinline__ void score_step(const Kv8AttnArgs& a, const Codes<NL>& k, const float (&vs)[2], const i32x4* qd,
+                                           float qmul, const Tile& t, int64_t pos, uint32_t step, float (&sc)[2][4]) {
   const uint32_t lane = threadIdx.x & 63;
   i32x4 acc[2][4];
   asm volatile("" ::: "memory");  // the digits are read in every step, not held
@@ -662,7 +667,7 @@ __device__ __forceinline__ void score_step(const Kv8AttnArgs& a, const Codes<NL>
       acc[1][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k.c[1][l], q, acc[1][d], 0, 0, 0);
     }
   }
-  finish_scores(a, acc, k.s, k.has, qmul, t, pos, step, sc);
+  finish_scores(a, acc, k.s, vs, k.has, qmul, t, pos, step, sc);
 }
 
 template <int NL>
@@ -851,7 +856,7 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   clear<NL>(&r);
   for (; s < s1; s += 4) {
     float sc[2][4];
-    score_step<NL>(a, k, qd, qmul, t, pos, s, sc);
+    score_step<NL>(a, k, v.s, qd, qmul, t, pos, s, sc);
     const bool more = s + 4 < s1;
     if (++i == 32 && more) {
       i = 0;
@@ -860,7 +865,7 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
     if (more) load_codes<NL, FULL, true>(a, t, s + 4, pages, i, &k);
     __builtin_amdgcn_sched_barrier(0);
     f16x8 hi, lo;
-    soft_step<NL>(sc, v.s, v.has, &r, &hi, &lo);
+    soft_step<NL, 0>(sc, v.s, v.has, &r, &hi, &lo);
     value_step<NL>(v, hi, lo, &r);
     if (more) load_codes<NL, FULL, false>(a, t, s + 4, pages, i, &v);
     __builtin_amdgcn_sched_barrier(0);
@@ -962,10 +967,10 @@ __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
   Tile mine = t;
   {
     const uint64_t p0 = t.past + min(c0, last) / G, p1 = t.past + min(c0 + KV8_COLS - 1, last) / G;
-    mine.lo = a.window && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
-    mine.hi = p1 + 1;
-    mine.all_lo = a.window && p1 + 1 > a.window ? p1 + 1 - a.window : 0;
-    mine.all_hi = p0 + 1;
+    mine.step0 = a.window && p0 + 1 > a.window ? (uint32_t)((p0 + 1 - a.window) / KV8_STEP) : 0;
+    mine.steps = (uint32_t)(p1 / KV8_STEP) + 1 - mine.step0;
+    mine.all0 = a.window && p1 + 1 > a.window ? (uint32_t)((p1 + KV8_STEP - a.window) / KV8_STEP) : 0;
+    mine.all1 = (uint32_t)((p0 + 1) / KV8_STEP);
   }
 
   uint32_t pages = step_pages(a, t, s0 + par, 2), at = 0;
@@ -1029,7 +1034,7 @@ __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
     if (s + 2 < s1) load(s + 2);
     __syncthreads();
     // (a step that none of the wave's columns sees: the others' barriers only)
-    if (s < s1 && (uint64_t)s * KV8_STEP < mine.hi && ((uint64_t)s + 1) * KV8_STEP > mine.lo) {
+    if (s < s1 && s - mine.step0 < mine.steps) {
       float sc[2][4];
       {
         i32x4 acc[2][4];
@@ -1045,13 +1050,13 @@ __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
             acc[1][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k1, q, acc[1][d], 0, 0, 0);
           }
         }
-        finish_scores(a, acc, ks, has, qmul, mine, pos, s, sc);
+        finish_scores(a, acc, ks, vs, has, qmul, mine, pos, s, sc);
       }
       f16x8 x[4];  // the values' operands, one l ahead
 #pragma unroll
       for (int j = 0; j < 4; j++) x[j] = vb[j * 64 + lane];
       f16x8 hi, lo;
-      soft_step<NL>(sc, vs, has, &r, &hi, &lo);
+      soft_step<NL, kLazy>(sc, vs, has, &r, &hi, &lo);
 #pragma unroll
       for (int l = 0; l < NL; l++) {
         f16x8 y[4];
@@ -1073,7 +1078,7 @@ __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
   r.l += __shfl_xor(r.l, 16, 64);
   r.l += __shfl_xor(r.l, 32, 64);
   // the odd steps' sums come to the wave of the even ones
-  float unit = r.E == kNoExp ? 0.f : ldexpf(1.f, r.E - 14);
+  float unit = r.E == kNoExp ? 0.f : ldexpf(1.f, r.E - (14 - kLazy));
   float* lm = reinterpret_cast<float*>(lds) + part * (16 * NL * 64 + 128);
   float* lo = lm + 128;
   if (par == 1) {

@@ -135,8 +135,9 @@ def attention(cache, rows, past, tables, q, scale, window):
     A score is a sum that the kernel has exactly, up to q's 31 bits, rounded a handful of times:
     |ds| <= 8 U |s|.  p = exp(s - max): relative error |ds| + |d max| + 4 U |s - max| + 4 U, P's two
     halves 4 U, the sums over n tokens and their joins (n / 4 + 64) U; the quotient has the sum's too.
-    The halves are f16 numbers in units of S / 2^14, S the largest V scale so far: what is left of p below
-    half their last step, 2^-25 units, is lost, times a code of up to 127 and over a sum of at least 1.
+    The halves are f16 numbers in units of S / 2^10 (few columns: 2^14), S the largest V scale so far: what
+    is left of p below half their last step, 2^-25 units, is lost, times a code of up to 127.  What is
+    subtracted from the scores is at least the maximum less 4 (log2), so the sum that divides is at least 1.
     """
     out, bound, at = np.zeros_like(q, np.float64), np.zeros_like(q, np.float64), 0
     G = q.shape[1] // cache.H
@@ -160,7 +161,7 @@ def attention(cache, rows, past, tables, q, scale, window):
                 out[at + i, h] = p @ vv
                 bound[at + i, h] = (p * rel) @ np.abs(vv) + (p @ rel) * np.abs(out[at + i, h])
                 at_most = np.nan_to_num(cache.scales[1][tables[b][tables[b] < cache.P]]).max()
-                bound[at + i, h] += len(p) * 127 * at_most * 2.0 ** -39
+                bound[at + i, h] += len(p) * 127 * at_most * 2.0 ** -35
         at += n
     return out, bound
 
