@@ -748,25 +748,30 @@ __device__ __forceinline__ float load_q(const Kv8AttnArgs& a, const float* q, i3
   return bad ? __builtin_nanf("") : ldexpf(1.f, e - 30);
 }
 
+// A wave's part of the query row q (dims 64 l + 16 g .. for every fourth l).
+template <int NL>
+__device__ __forceinline__ void load_row(const float* q, uint32_t D, f32x4 (&x)[(NL + 3) / 4][4]) {
+  const uint32_t g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int i = 0; i < (NL + 3) / 4; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint32_t d = 64 * (wave_id() + 4 * i) + 16 * g + 4 * j;
+      x[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (d < D) x[i][j] = *reinterpret_cast<const f32x4*>(q + d);
+    }
+}
+
 // The tile's query columns as digits in LDS, qd[digit][l][lane] (dims 64 l + 16 g
 // .. of column n); a wave makes every fourth l.  A row's largest magnitude (joined
 // through qm) decides its unit, which is returned (NaN where the row has a NaN or
 // an infinity).
 template <int NL>
-__device__ __forceinline__ float stage_q(const Kv8AttnArgs& a, const float* q, float* qm, i32x4* qd) {
+__device__ __forceinline__ float stage_q(const f32x4 (&x)[(NL + 3) / 4][4], float* qm, i32x4* qd) {
   constexpr int NS = (NL + 3) / 4;
-  const uint32_t lane = threadIdx.x & 63, wave = wave_id(), n = lane & 15, g = lane >> 4, D = a.c.D;
-  f32x4 x[NS][4];
+  const uint32_t lane = threadIdx.x & 63, wave = wave_id(), n = lane & 15;
   float amax = 0.f;
   bool bad = false;
-#pragma unroll
-  for (int i = 0; i < NS; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const uint32_t d = 64 * (wave + 4 * i) + 16 * g + 4 * j;
-      x[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (d < D) x[i][j] = *reinterpret_cast<const f32x4*>(q + d);
-    }
 #pragma unroll
   for (int i = 0; i < NS; i++)
 #pragma unroll
@@ -807,17 +812,19 @@ __device__ __forceinline__ float stage_q(const Kv8AttnArgs& a, const float* q, f
   return bad ? __builtin_nanf("") : ldexpf(1.f, e - 30);
 }
 
-// A lane's sums of its column (dims 64 l + 16 g + 4 i .. for each l, i), times by.
-template <int NL>
-__device__ __forceinline__ void write_column(const Run<NL>& r, float* to, uint32_t D, float by) {
+// A lane's sums of its column (dims d0 + 16 g + 4 i .. for each i), times by.
+__device__ __forceinline__ void write_dims(const f32x4 (&o)[4], float* to, uint32_t d0, uint32_t D, float by) {
   const uint32_t g = (threadIdx.x & 63) >> 4;
 #pragma unroll
-  for (int l = 0; l < NL; l++)
+  for (int i = 0; i < 4; i++) {
+    const uint32_t d = d0 + 16 * g + 4 * i;
+    if (d < D) *reinterpret_cast<f32x4*>(to + d) = f32x4{o[0][i], o[1][i], o[2][i], o[3][i]} * by;
+  }
+}
+template <int NL>
+__device__ __forceinline__ void write_column(const Run<NL>& r, float* to, uint32_t D, float by) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t d = 64 * l + 16 * g + 4 * i;
-      if (d < D) *reinterpret_cast<f32x4*>(to + d) = f32x4{r.o[l][0][i], r.o[l][1][i], r.o[l][2][i], r.o[l][3][i]} * by;
-    }
+  for (int l = 0; l < NL; l++) write_dims(r.o[l], to, 64 * l, D, by);
 }
 
 // Few query columns (one tile): the workgroup's waves take its steps in turn.  The
@@ -841,9 +848,12 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   float* lm = reinterpret_cast<float*>(lds);         // [4][16]
   float* ll = lm + 64;                               // [4][16]
   i32x4* qd = reinterpret_cast<i32x4*>(lds + 512);   // [4][NL][64]
-  float* lo = reinterpret_cast<float*>(lds + 512);   // [2 waves][16 NL floats][64 lanes], after the steps
+  f32x4* lo = reinterpret_cast<f32x4*>(lds + 512);   // [4 waves][NL][4][64 lanes], after the steps
   uint32_t pages = step_pages(a, t, s0 + wave, 4);
   const uint32_t col = t.col0 + min(n, t.ncol - 1);  // columns past the last repeat it
+  f32x4 row[(NL + 3) / 4][4];
+  load_row<NL>(a.q + row_at(a, t, col), D, row);
+  __builtin_amdgcn_sched_barrier(0);
   const int64_t pos = (int64_t)(t.past + col / G);
   Codes<NL> k, v;
   uint32_t i = 0, s = s0 + wave;
@@ -851,7 +861,7 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
     load_codes<NL, FULL, true>(a, t, s, pages, 0, &k);
     load_codes<NL, FULL, false>(a, t, s, pages, 0, &v);
   }
-  const float qmul = stage_q<NL>(a, a.q + row_at(a, t, col), lm, qd) * (a.scale * kLog2e);
+  const float qmul = stage_q<NL>(row, lm, qd) * (a.scale * kLog2e);
   Run<NL> r;
   clear<NL>(&r);
   for (; s < s1; s += 4) {
@@ -873,7 +883,7 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   r.l += __shfl_xor(r.l, 16, 64);
   r.l += __shfl_xor(r.l, 32, 64);
 
-  // join the waves: m and l of all, then o by a tree through LDS
+  // Join the waves: m and l of all, then each wave the sums of a quarter of the dims.
   if (lane < 16) {
     lm[wave * 16 + n] = r.m;
     ll[wave * 16 + n] = r.l;
@@ -889,31 +899,9 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
 #pragma unroll
   for (int l = 0; l < NL; l++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) r.o[l][j] *= fe;
-#pragma unroll
-  for (int half = 2; half >= 1; half >>= 1) {
-    if (wave >= half && wave < 2 * half) {
-      float* to = lo + (wave - half) * (16 * NL * 64);
-#pragma unroll
-      for (int l = 0; l < NL; l++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) to[(l * 16 + j * 4 + i) * 64 + lane] = r.o[l][j][i];
-    }
-    __syncthreads();
-    if (wave < half) {
-      const float* from = lo + wave * (16 * NL * 64);
-#pragma unroll
-      for (int l = 0; l < NL; l++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) r.o[l][j][i] += from[(l * 16 + j * 4 + i) * 64 + lane];
-    }
-    __syncthreads();
-  }
-  if (wave != 0 || n >= t.ncol) return;
+    for (int j = 0; j < 4; j++) lo[((wave * NL + l) * 4 + j) * 64 + lane] = r.o[l][j] * fe;
+  __syncthreads();
+  if (n >= t.ncol) return;
   const bool only = per >= t.steps;  // the only split that runs
   float* to;
   float by = 1.f;
@@ -923,12 +911,24 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   } else {
     const uint64_t unit = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / a.nsplit) + tile;
     to = a.part + ((unit * a.nsplit + split) * KV8_COLS + n) * (D + KV8_PART);
-    if (g == 0) {
+    if (wave == 0 && g == 0) {
       to[D] = M;
       to[D + 1] = L;
     }
   }
-  write_column<NL>(r, to, D, by);
+#pragma unroll
+  for (int i = 0; i < (NL + 3) / 4; i++) {
+    const uint32_t l = wave + 4 * i;
+    if (l >= NL) break;
+    f32x4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      x[j] = lo[(l * 4 + j) * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < 4; w++) x[j] += lo[((w * NL + l) * 4 + j) * 64 + lane];
+    }
+    write_dims(x, to, 64 * l, D, by);
+  }
 }
 
 // Many query columns (a prompt's).  The matrix instructions bound it (per step and

@@ -113,7 +113,7 @@ gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, co
   if (window) tokens = std::min<uint64_t>(tokens, (uint64_t)window + (p->width + G - 1) / G);
   const uint64_t steps = tokens / KV8_STEP + 1, units = tiles * c.nkv * r.num_seqs;
   const uint64_t most = std::min<uint64_t>((steps + p->chunk - 1) / p->chunk, KV8_MAX_SPLIT);
-  const uint64_t want = p->rows ? 2ull * ctx->num_cus / units : (2ull * ctx->num_cus + units - 1) / units;
+  const uint64_t want = 2ull * ctx->num_cus / units;
   p->nsplit = (uint32_t)std::max<uint64_t>(1, std::min(want, most));
   p->chunk = (uint32_t)std::max<uint64_t>(p->chunk, (steps + p->nsplit - 1) / p->nsplit);
   if (tiles * p->nsplit * c.nkv > 0x7fffffffull || tiles * p->width > 0x7fffffffull) return unsupported(who, "too many query rows");
@@ -265,7 +265,7 @@ gh_status gh_kv8_attn(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8_b
                              (a.c.D == 64 * nl ? "_k" : "r_k");
     void* args[] = {&a};
     st = p.rows ? launch(ctx, name.c_str(), dim3(p.tiles * p.nsplit * a.c.nkv, 1, a.b.num_seqs), dim3(256), 14336 * nl, args)
-                : launch(ctx, name.c_str(), dim3(p.tiles * p.nsplit, a.c.nkv, a.b.num_seqs), dim3(256), 512 + 8192 * nl, args);
+                : launch(ctx, name.c_str(), dim3(p.tiles * p.nsplit, a.c.nkv, a.b.num_seqs), dim3(256), 512 + 16384 * nl, args);
     if (st != GH_OK || p.nsplit == 1) return st;
     uint32_t cols = (uint32_t)std::min<uint64_t>(p.width, (uint64_t)a.b.max_rows * (num_q / a.c.nkv));
     void* margs[] = {&a, &p.width, &cols};
