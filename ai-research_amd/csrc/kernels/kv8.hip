@@ -821,11 +821,6 @@ __device__ __forceinline__ void write_dims(const f32x4 (&o)[4], float* to, uint3
     if (d < D) *reinterpret_cast<f32x4*>(to + d) = f32x4{o[0][i], o[1][i], o[2][i], o[3][i]} * by;
   }
 }
-template <int NL>
-__device__ __forceinline__ void write_column(const Run<NL>& r, float* to, uint32_t D, float by) {
-#pragma unroll
-  for (int l = 0; l < NL; l++) write_dims(r.o[l], to, 64 * l, D, by);
-}
 
 // Few query columns (one tile): the workgroup's waves take its steps in turn.  The
 // tokens' bytes bound it, so a wave has the next step's keys on the way while it
@@ -941,8 +936,8 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
 // together).  The codes of a step come through LDS once for its two waves, the values'
 // already as f16, whose conversion is as much vector work as the softmax; the next
 // step's are on their way to registers meanwhile.
-// grid (tiles * splits * kv heads, 1, sequences), the tiles that see most first; the
-// heads in turn, so that with eight of them a head's workgroups share an XCD's L2.
+// grid (tiles * kv heads, 1, sequences), the tiles that see most first; the heads in
+// turn, so that with eight of them a head's workgroups share an XCD's L2.
 template <int NL, bool FULL>
 __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
   extern __shared__ __align__(16) char lds[];
@@ -950,14 +945,11 @@ __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
   constexpr uint32_t kPieces = 2 * NL * 64, vPieces = 4 * NL * 64;  // 16 bytes each, of a step
   const uint32_t lane = threadIdx.x & 63, wave = wave_id(), n = lane & 15, g = lane >> 4;
   const uint32_t part = wave & 1, par = wave >> 1;
-  const uint32_t D = FULL ? 64 * NL : a.c.D, G = a.nq / a.c.nkv, each = a.c.nkv * a.nsplit, tiles = gridDim.x / each;
-  const uint32_t head = blockIdx.x % a.c.nkv, split = blockIdx.x / a.c.nkv % a.nsplit, tile = tiles - 1 - blockIdx.x / each;
+  const uint32_t D = FULL ? 64 * NL : a.c.D, G = a.nq / a.c.nkv;
+  const uint32_t head = blockIdx.x % a.c.nkv, tile = gridDim.x / a.c.nkv - 1 - blockIdx.x / a.c.nkv;
   Tile t;
   if (!tile_of(a, blockIdx.z, head, tile, KV8_ROW_COLS, &t)) return;
-  const uint32_t per = kv8_split_steps(t.steps, a.nsplit, a.chunk);
-  const uint32_t s0 = t.step0 + split * per, end = t.step0 + t.steps;
-  if (split > 0 && s0 >= end) return;
-  const uint32_t s1 = min(s0 + per, end);
+  const uint32_t s0 = t.step0, s1 = t.step0 + t.steps;
   i32x4* kb = reinterpret_cast<i32x4*>(lds) + par * (kPieces + vPieces);
   f16x8* vb = reinterpret_cast<f16x8*>(kb + kPieces);
 
@@ -1104,17 +1096,10 @@ __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
 #pragma unroll
       for (int i = 0; i < 4; i++) r.o[l][j][i] = fmaf(lo[(l * 16 + j * 4 + i) * 64 + lane], f1, r.o[l][j][i] * unit);
   if (c0 + n > last) return;
-  if (per >= t.steps) {  // the only split that runs; nothing visible: 0
-    write_column<NL>(r, a.out + row_at(a, t, col), D, M == -INFINITY && L == 0.f ? 0.f : 1.f / L);
-  } else {
-    const uint64_t place = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * tiles + tile;
-    float* to = a.part + ((place * a.nsplit + split) * KV8_ROW_COLS + (col - t.col0)) * (D + KV8_PART);
-    if (g == 0) {
-      to[D] = M;
-      to[D + 1] = L;
-    }
-    write_column<NL>(r, to, D, 1.f);
-  }
+  const float by = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;  // nothing visible: 0
+  float* to = a.out + row_at(a, t, col);
+#pragma unroll
+  for (int l = 0; l < NL; l++) write_dims(r.o[l], to, 64 * l, D, by);
 }
 
 }  // namespace
@@ -1135,16 +1120,15 @@ KV8_ATTN(8, 1)
 
 // Joins the splits of a tile's column, in split order: the splits' factors in
 // LDS, then a lane a dim.  grid (tiles * columns a tile can have, kv heads, sequences)
-extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, uint32_t width,
-                                                                           uint32_t cols) {
+extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, uint32_t cols) {
   const uint32_t tile = blockIdx.x / cols, n = blockIdx.x % cols, D = a.c.D;
   Tile t;
-  if (!tile_of(a, blockIdx.z, blockIdx.y, tile, width, &t) || n >= t.ncol) return;
+  if (!tile_of(a, blockIdx.z, blockIdx.y, tile, KV8_COLS, &t) || n >= t.ncol) return;
   const uint32_t per = kv8_split_steps(t.steps, a.nsplit, a.chunk);
   if (per >= t.steps) return;  // written by its only split
   const uint32_t live = (t.steps + per - 1) / per, tid = threadIdx.x;
   const uint64_t unit = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / cols) + tile;
-  const uint64_t row = width * (uint64_t)(D + KV8_PART);
+  const uint64_t row = KV8_COLS * (uint64_t)(D + KV8_PART);
   const float* p = a.part + unit * a.nsplit * row + n * (uint64_t)(D + KV8_PART);
   __shared__ float f[KV8_MAX_SPLIT], red[8];
   float m = -INFINITY, l = 0.f;

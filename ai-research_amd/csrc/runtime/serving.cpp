@@ -84,41 +84,62 @@ bool empty(const Kv8Rows& r) { return r.num_seqs == 0 || r.num_rows == 0 || r.ma
 // Blocks that a sequence's rows can touch.
 uint32_t touched(const Kv8Rows& r) { return (r.max_rows + KV8_BLOCK - 2) / KV8_BLOCK + 1; }
 
+// Of heads of up to 64 nl dims the kernels have variants.
+uint32_t dims64(const Kv8View& c) { return c.D <= 64 ? 1 : c.D <= 128 ? 2 : c.D <= 256 ? 4 : 8; }
+
 struct AttnPlan {
   bool rows = false;  // the kernel of many columns
-  uint32_t width = KV8_COLS, tiles = 0, nsplit = 1, chunk = 4;
+  uint32_t tiles = 0, nsplit = 1, chunk = 1;
   size_t bytes = 0;
 };
 
-// Splits of the token range, of equal length in tokens, so that long sequences of
-// a batch take more of them than short ones: as many as give every CU the two
-// workgroups it holds.  More of them cost more in starts than they balance: 32
-// sequences of 20 - 4000 tokens take 71 us with two a CU, 80 with four, 94 with
-// eight, one of 120000 103 / 112 / 129.  A split takes at least a step for each of
-// its four waves.
+// Which kernel, and into how many parts each sequence's tokens are split.
+//
+// The kernel of many columns halves what is read and converted a column, and wants many
+// workgroups: it is taken where tiles of 16 columns alone give every CU two of them.
+// (us with it and with the other one, 8 key heads of 256 under 16 query heads: prompts
+// of 2000 tokens 98 / 120, 700: 31 / 32, 8 of 64 rows over 1000: 41 / 47, over 4000: 123
+// / 158; with fewer tiles, a prompt of 500: 24 / 20, 8 of 32 over 2000: 47 / 45.)
+//
+// The other one splits the tokens where that shortens the whole: its four waves take
+// steps of 32 tokens in turn, 2.3 us for a step each (256 dims; 0.6 more of that for
+// every workgroup a CU has beyond one), and the splits' sums cost a launch and their
+// way through memory, 4 us and 3 TB/s.  (One token over 544, 8 heads: 5 splits 12 us,
+// none 19; 8 sequences of 32 rows over 2000, 256 tiles: none 45, 2 58; a prompt of 256
+// tokens, 256 tiles: none 11, 2 22; 32 sequences of 20 - 4000 tokens, 256 tiles: 2 67,
+// none 76.)  Parts are of equal length in tokens, so that long sequences of a batch
+// take more of them than short ones, and at most as many as two a CU.
 gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, const Kv8Rows& r, uint32_t num_q,
                     uint32_t window, uint32_t max_kv, AttnPlan* p) {
   if (num_q == 0 || num_q % c.nkv) return invalid(who, "num_q must be a positive multiple of the kv heads");
   if (num_q > 65536) return unsupported(who, "more than 65536 query heads");
   *p = AttnPlan{};
   if (empty(r)) return GH_OK;
-  const uint64_t G = num_q / c.nkv, cols = r.max_rows * G;
-  static const uint64_t row_min = getenv("KV8_ROWMIN") ? atoi(getenv("KV8_ROWMIN")) : 33;
-  p->rows = cols >= row_min;
-  if (p->rows) p->width = KV8_ROW_COLS;
-  if (p->rows) p->chunk = getenv("KV8_CHUNK") ? atoi(getenv("KV8_CHUNK")) : 16;
-  const uint64_t tiles = (cols + p->width - 1) / p->width;
+  const uint64_t G = num_q / c.nkv, cols = r.max_rows * G, cus = std::max(ctx->num_cus, 1);
+  uint64_t tiles = (cols + KV8_COLS - 1) / KV8_COLS, units = tiles * c.nkv * r.num_seqs;
+  p->rows = units >= 2 * cus;
+  if (p->rows) tiles = (cols + KV8_ROW_COLS - 1) / KV8_ROW_COLS;
+  if (tiles * c.nkv > 0x7fffffffull || tiles * KV8_ROW_COLS > 0x7fffffffull) return unsupported(who, "too many query rows");
+  p->tiles = (uint32_t)tiles;
+  if (p->rows) return GH_OK;
   uint64_t tokens = (uint64_t)r.max_pages << c.page_shift;
   if (max_kv) tokens = std::min<uint64_t>(tokens, max_kv);
-  if (window) tokens = std::min<uint64_t>(tokens, (uint64_t)window + (p->width + G - 1) / G);
-  const uint64_t steps = tokens / KV8_STEP + 1, units = tiles * c.nkv * r.num_seqs;
-  const uint64_t most = std::min<uint64_t>((steps + p->chunk - 1) / p->chunk, KV8_MAX_SPLIT);
-  const uint64_t want = 2ull * ctx->num_cus / units;
-  p->nsplit = (uint32_t)std::max<uint64_t>(1, std::min(want, most));
-  p->chunk = (uint32_t)std::max<uint64_t>(p->chunk, (steps + p->nsplit - 1) / p->nsplit);
-  if (tiles * p->nsplit * c.nkv > 0x7fffffffull || tiles * p->width > 0x7fffffffull) return unsupported(who, "too many query rows");
-  p->tiles = (uint32_t)tiles;
-  if (p->nsplit > 1) p->bytes = (size_t)units * p->nsplit * p->width * (c.D + KV8_PART) * sizeof(float);
+  if (window) tokens = std::min<uint64_t>(tokens, (uint64_t)window + (KV8_COLS + G - 1) / G);
+  const uint64_t steps = tokens / KV8_STEP + 1;
+  const uint64_t most = std::min<uint64_t>({(steps + 3) / 4, 2 * cus / units, KV8_MAX_SPLIT});
+  double least = INFINITY;
+  for (uint64_t n = 1; n <= std::max<uint64_t>(most, 1); n++) {
+    const double turns = (double)(((steps + n - 1) / n + 3) / 4), each = 2.3 * std::max(0.5, c.D / 256.0);
+    const double load = std::max(1.0, 1 + 0.6 * ((double)(units * n) / (double)cus - 1));
+    const double join = n > 1 ? 4 + (double)(units * n) * c.D * (2 * sizeof(float) * KV8_COLS) / 3e6 : 0;
+    const double us = turns * each * load + join;
+    if (us < least) {
+      least = us;
+      p->nsplit = (uint32_t)n;
+    }
+  }
+  p->chunk = (uint32_t)((steps + p->nsplit - 1) / p->nsplit);
+  if (p->nsplit > 1) p->bytes = (size_t)units * p->nsplit * KV8_COLS * (c.D + KV8_PART) * sizeof(float);
   return GH_OK;
 }
 
@@ -259,16 +280,16 @@ gh_status gh_kv8_attn(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8_b
     a.nsplit = p.nsplit;
     a.chunk = p.chunk;
     a.scale = scale;
-    const uint32_t nl = a.c.D <= 64 ? 1 : a.c.D <= 128 ? 2 : a.c.D <= 256 ? 4 : 8;
+    const uint32_t nl = dims64(a.c);
     // r: heads of fewer dims than the kernel's 64 nl
     const std::string name = std::string(p.rows ? "gh_kv8_rows_l" : "gh_kv8_attn_l") + std::to_string(nl) +
                              (a.c.D == 64 * nl ? "_k" : "r_k");
     void* args[] = {&a};
-    st = p.rows ? launch(ctx, name.c_str(), dim3(p.tiles * p.nsplit * a.c.nkv, 1, a.b.num_seqs), dim3(256), 14336 * nl, args)
-                : launch(ctx, name.c_str(), dim3(p.tiles * p.nsplit, a.c.nkv, a.b.num_seqs), dim3(256), 512 + 16384 * nl, args);
+    if (p.rows) return launch(ctx, name.c_str(), dim3(p.tiles * a.c.nkv, 1, a.b.num_seqs), dim3(256), 14336 * nl, args);
+    st = launch(ctx, name.c_str(), dim3(p.tiles * p.nsplit, a.c.nkv, a.b.num_seqs), dim3(256), 512 + 16384 * nl, args);
     if (st != GH_OK || p.nsplit == 1) return st;
-    uint32_t cols = (uint32_t)std::min<uint64_t>(p.width, (uint64_t)a.b.max_rows * (num_q / a.c.nkv));
-    void* margs[] = {&a, &p.width, &cols};
+    uint32_t cols = (uint32_t)std::min<uint64_t>(KV8_COLS, (uint64_t)a.b.max_rows * (num_q / a.c.nkv));
+    void* margs[] = {&a, &cols};
     return launch(ctx, "gh_kv8_merge_k", dim3(p.tiles * cols, a.c.nkv, a.b.num_seqs), dim3(256), 0, margs);
   });
 }

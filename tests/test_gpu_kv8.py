@@ -249,6 +249,17 @@ def run_attn(gpu, dev, rows, past, tables, q, scale, window, max_kv=0, **bounds)
     return O.read(np.float32).reshape(q.shape)
 
 
+def run_many(gpu, dev, rows, past, tables, q, scale, window, max_kv=0, **bounds):
+    """The same as the head of a batch with room for many more rows: the kernel of many columns."""
+    room = np.full((q.shape[0] + 10000 // q.shape[1], *q.shape[1:]), np.nan, np.float32)
+    room[:len(q)] = q
+    many = dict(num_rows=len(room), max_rows=len(room)) if not bounds else bounds
+    got = run_attn(gpu, dev, rows, past, tables, room, scale, window, max_kv, **many)
+    assert np.all(got[len(q):] == 5.0)
+    return got[:len(q)]
+
+
+RUNS = pytest.mark.parametrize("run", [run_attn, run_many])
 ATTN = [  # nq, H, D, page, rows, past, window, scale
     (16, 8, 256, 16, [1], [543], 0, 1.0),
     (16, 8, 256, 32, [1, 1, 1, 1, 0, 1], [0, 15, 16, 700, 40, 129], 0, 0.0625),
@@ -269,7 +280,8 @@ ATTN = [  # nq, H, D, page, rows, past, window, scale
 
 
 @pytest.mark.parametrize("nq,H,D,page,rows,past,window,scale", ATTN)
-def test_attention(gpu, nq, H, D, page, rows, past, window, scale):
+@RUNS
+def test_attention(gpu, run, nq, H, D, page, rows, past, window, scale):
     rng = np.random.default_rng(nq * D + page + window)
     per = max(-(-(p + r) // page) for p, r in zip(past, rows)) + 1
     cache = ref.Cache(len(rows) * per + 2, page, H, D, rng)
@@ -278,11 +290,12 @@ def test_attention(gpu, nq, H, D, page, rows, past, window, scale):
     q = rng.standard_normal((sum(rows), nq, D)).astype(np.float32)
     want, bound = ref.attention(cache, rows, past, tables, q, scale, window)
     for max_kv in (0, max(p + r for p, r in zip(past, rows)), 1):  # (a plan for less than there is computes the same)
-        got = run_attn(gpu, dev, rows, past, tables, q, scale, window, max_kv)
+        got = run(gpu, dev, rows, past, tables, q, scale, window, max_kv)
         assert np.all(np.abs(got - want) <= bound), float((np.abs(got - want) / bound).max())
 
 
-def test_attention_scales_far_apart_and_zero_blocks(gpu):
+@RUNS
+def test_attention_scales_far_apart_and_zero_blocks(gpu, run):
     # V blocks whose scales differ by 2^40: small probabilities times large values count
     nq, H, D, page = 4, 2, 128, 16
     rng = np.random.default_rng(12)
@@ -296,11 +309,12 @@ def test_attention_scales_far_apart_and_zero_blocks(gpu):
     tables = np.arange(12, dtype=np.uint32)[None]
     q = rng.standard_normal((1, nq, D)).astype(np.float32) * 0.3
     want, bound = ref.attention(cache, [1], [180], tables, q, 0.1, 0)
-    got = run_attn(gpu, dev, [1], [180], tables, q, 0.1, 0)
+    got = run(gpu, dev, [1], [180], tables, q, 0.1, 0)
     assert np.all(np.abs(got - want) <= bound)
 
 
-def test_attention_masked_places_may_hold_anything(gpu):
+@RUNS
+def test_attention_masked_places_may_hold_anything(gpu, run):
     # NaN, infinite and huge scales behind a sequence's last token, in front of its window and in
     # pages of others change nothing; pages that are absent are as masked
     nq, H, D, page = 4, 2, 64, 32
@@ -317,11 +331,12 @@ def test_attention_masked_places_may_hold_anything(gpu):
         s[1], s[6] = np.nan, np.inf        # behind both ends
         s[7, :, 1] = 2.0 ** 120            # tokens 80 .. 95 of the first sequence
     dev = ref.Device(gpu, cache)
-    got = run_attn(gpu, dev, rows, past, tables, q, 0.2, window)
+    got = run(gpu, dev, rows, past, tables, q, 0.2, window)
     assert np.all(np.abs(got - want) <= bound)
 
 
-def test_attention_rows_that_see_nothing(gpu):
+@RUNS
+def test_attention_rows_that_see_nothing(gpu, run):
     nq, H, D, page = 2, 1, 64, 16
     rng = np.random.default_rng(2)
     cache = ref.Cache(2, page, H, D, rng)
@@ -329,18 +344,19 @@ def test_attention_rows_that_see_nothing(gpu):
     q = rng.standard_normal((4, nq, D)).astype(np.float32)
     tables = np.array([[0xffffffff, 0xffffffff], [9, 1]], np.uint32)
     # first: no page at all; second: window 2 at tokens 40, 41, past the table
-    got = run_attn(gpu, dev, [2, 2], [0, 40], tables, q, 1.0, 2)
+    got = run(gpu, dev, [2, 2], [0, 40], tables, q, 1.0, 2)
     assert not got.any()
     # rows of no sequence and rows over the bounds keep what they have
-    got = run_attn(gpu, dev, [2], [3], np.array([[1, 0]], np.uint32), q, 1.0, 0, num_rows=4)
+    got = run(gpu, dev, [2], [3], np.array([[1, 0]], np.uint32), q, 1.0, 0, num_rows=4)
     assert np.all(got[2:] == 5.0) and not np.any(got[:2] == 5.0)
-    got = run_attn(gpu, dev, [4], [3], np.array([[1, 0]], np.uint32), q, 1.0, 0, max_rows=1)
+    got = run(gpu, dev, [4], [3], np.array([[1, 0]], np.uint32), q, 1.0, 0, max_rows=1)
     assert np.all(got[1:] == 5.0)
-    got = run_attn(gpu, dev, [0, 0], [3, 1], np.array([[1, 0], [0, 1]], np.uint32), q, 1.0, 0, num_rows=4, max_rows=4)
+    got = run(gpu, dev, [0, 0], [3, 1], np.array([[1, 0], [0, 1]], np.uint32), q, 1.0, 0, num_rows=4, max_rows=4)
     assert np.all(got == 5.0)
 
 
-def test_attention_queries_of_any_size(gpu):
+@RUNS
+def test_attention_queries_of_any_size(gpu, run):
     # rows of zeros, tiny, huge and broken queries next to ordinary ones
     nq, H, D, page = 2, 1, 128, 16
     rng = np.random.default_rng(6)
@@ -354,13 +370,14 @@ def test_attention_queries_of_any_size(gpu):
     q[4, 0, 3] = np.nan
     q[4, 1, 5] = np.inf
     want, bound = ref.attention(cache, [6], [50], tables, np.nan_to_num(q, posinf=0), 0.05, 0)
-    got = run_attn(gpu, dev, [6], [50], tables, q, 0.05, 0)
+    got = run(gpu, dev, [6], [50], tables, q, 0.05, 0)
     assert np.isnan(got[4]).all()
     fine = [0, 1, 2, 3, 5]
     assert np.all(np.abs(got - want)[fine] <= bound[fine])
 
 
-def test_attention_nan_block_spoils_its_rows_only(gpu):
+@RUNS
+def test_attention_nan_block_spoils_its_rows_only(gpu, run):
     nq, H, D, page = 4, 2, 64, 16
     rng = np.random.default_rng(16)
     cache = ref.Cache(8, page, H, D, rng)
@@ -369,9 +386,33 @@ def test_attention_nan_block_spoils_its_rows_only(gpu):
     want, bound = ref.attention(cache, [1, 1], [60, 60], tables, q, 0.2, 0)
     cache.scales[0][2, 1] = np.nan
     dev = ref.Device(gpu, cache)
-    got = run_attn(gpu, dev, [1, 1], [60, 60], tables, q, 0.2, 0)
+    got = run(gpu, dev, [1, 1], [60, 60], tables, q, 0.2, 0)
     assert np.isnan(got[0, 2:]).all()
     assert np.all(np.abs(got - want)[0, :2] <= bound[0, :2]) and np.all(np.abs(got - want)[1] <= bound[1])
+
+
+@pytest.mark.parametrize("nq,H,D,page,rows,past,window,scale", [
+    (8, 8, 64, 64, [1100], [0], 0, 0.125),
+    (8, 8, 64, 16, [1100], [40], 100, 0.125),
+    (8, 4, 48, 32, [600, 3, 0, 700], [0, 500, 7, 33], 0, 0.15),
+    (16, 2, 272, 32, [1030], [5], 0, 0.06),
+])
+def test_attention_of_long_prompts(gpu, nq, H, D, page, rows, past, window, scale):
+    rng = np.random.default_rng(D + window)
+    per = max(-(-(p + r) // page) for p, r in zip(past, rows))
+    cache = ref.Cache(len(rows) * per, page, H, D, rng)
+    dev = ref.Device(gpu, cache)
+    tables = tables_of(rng, len(rows), per, cache.P)
+    q = rng.standard_normal((sum(rows), nq, D)).astype(np.float32)
+    got = run_attn(gpu, dev, rows, past, tables, q, scale, window)
+    assert gpu.kv8_attn_workspace(dev.cache, dev.batch(rows, past, tables), nq, window, 0) == 0
+    # (every seventh row: a batch of its own to the formula)
+    at = 0
+    for b, n in enumerate(rows):
+        for i in list(range(0, n, 7)) + [n - 1] * (n > 0):
+            want, bound = ref.attention(cache, [1], [past[b] + i], tables[b:b + 1], q[at + i:at + i + 1], scale, window)
+            assert np.all(np.abs(got[at + i:at + i + 1] - want) <= bound), (b, i)
+        at += n
 
 
 def test_attention_repeats_and_replays(gpu):
