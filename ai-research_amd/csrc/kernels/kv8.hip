@@ -260,8 +260,7 @@ __device__ __forceinline__ void append_kv(const Kv8AppendArgs& a, Angle* ang, in
     __syncthreads();
   }
 
-  double x0[4][NP], x1[4][NP], ss[4], amax = 0.0;
-  bool bad = false;
+  double x0[4][NP], x1[4][NP], ss[4], amax = 0.0, odd = 0.0;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
     const uint32_t t = wave * 4 + j;
@@ -300,13 +299,12 @@ __device__ __forceinline__ void append_kv(const Kv8AppendArgs& a, Angle* ang, in
       }
       x0[j][m] = u;
       x1[j][m] = w;
-      amax = fabs(u) > amax ? fabs(u) : amax;
-      amax = fabs(w) > amax ? fabs(w) : amax;
-      bad |= !(fabs(u) < 1e300) || !(fabs(w) < 1e300);
+      amax = fmax(amax, fmax(fabs(u), fabs(w)));
+      odd = fma(u, 0.0, fma(w, 0.0, odd));  // NaN once there is a NaN or an infinity
     }
   }
   amax = wave_max(amax);
-  if (__any(bad)) amax = HUGE_VAL;
+  if (__any(odd != odd)) amax = HUGE_VAL;
   if (lane == 0) red[wave] = amax;
   __syncthreads();
   amax = fmax(fmax(red[0], red[1]), fmax(red[2], red[3]));
@@ -890,11 +888,12 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
   for (int w = 0; w < 4; w++) L += ll[w * 16 + n] * __builtin_amdgcn_exp2f(lm[w * 16 + n] - base);
-  const float f = __builtin_amdgcn_exp2f(r.m - base), fe = r.E == kNoExp ? 0.f : ldexpf(f, r.E - 14);
+  // (two factors: the unit of the smallest scales is below f32's normal range)
+  const float f = __builtin_amdgcn_exp2f(r.m - base), unit = r.E == kNoExp ? 0.f : ldexpf(1.f, r.E - 14);
 #pragma unroll
   for (int l = 0; l < NL; l++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) lo[((wave * NL + l) * 4 + j) * 64 + lane] = r.o[l][j] * fe;
+    for (int j = 0; j < 4; j++) lo[((wave * NL + l) * 4 + j) * 64 + lane] = r.o[l][j] * f * unit;
   __syncthreads();
   if (n >= t.ncol) return;
   const bool only = per >= t.steps;  // the only split that runs
@@ -904,8 +903,8 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
     to = a.out + row_at(a, t, col);
     by = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;  // nothing visible: 0
   } else {
-    const uint64_t unit = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / a.nsplit) + tile;
-    to = a.part + ((unit * a.nsplit + split) * KV8_COLS + n) * (D + KV8_PART);
+    const uint64_t place = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / a.nsplit) + tile;
+    to = a.part + ((place * a.nsplit + split) * KV8_COLS + n) * (D + KV8_PART);
     if (wave == 0 && g == 0) {
       to[D] = M;
       to[D + 1] = L;
@@ -1070,7 +1069,7 @@ __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
   r.l += __shfl_xor(r.l, 16, 64);
   r.l += __shfl_xor(r.l, 32, 64);
   // the odd steps' sums come to the wave of the even ones
-  float unit = r.E == kNoExp ? 0.f : ldexpf(1.f, r.E - (14 - kLazy));
+  const float unit = r.E == kNoExp ? 0.f : ldexpf(1.f, r.E - (14 - kLazy));
   float* lm = reinterpret_cast<float*>(lds) + part * (16 * NL * 64 + 128);
   float* lo = lm + 128;
   if (par == 1) {
@@ -1088,13 +1087,12 @@ __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
   const float m1 = lm[lane], M = fmaxf(r.m, m1), base = M == -INFINITY ? 0.f : M;
   const float f0 = __builtin_amdgcn_exp2f(r.m - base), f1 = __builtin_amdgcn_exp2f(m1 - base);
   const float L = r.l * f0 + lm[64 + lane] * f1;
-  unit *= f0;
 #pragma unroll
   for (int l = 0; l < NL; l++)
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) r.o[l][j][i] = fmaf(lo[(l * 16 + j * 4 + i) * 64 + lane], f1, r.o[l][j][i] * unit);
+      for (int i = 0; i < 4; i++) r.o[l][j][i] = fmaf(lo[(l * 16 + j * 4 + i) * 64 + lane], f1, r.o[l][j][i] * f0 * unit);
   if (c0 + n > last) return;
   const float by = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;  // nothing visible: 0
   float* to = a.out + row_at(a, t, col);

@@ -119,7 +119,8 @@ gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, co
   uint64_t tiles = (cols + KV8_COLS - 1) / KV8_COLS, units = tiles * c.nkv * r.num_seqs;
   p->rows = units >= 2 * cus;
   if (p->rows) tiles = (cols + KV8_ROW_COLS - 1) / KV8_ROW_COLS;
-  if (tiles * c.nkv > 0x7fffffffull || tiles * KV8_ROW_COLS > 0x7fffffffull) return unsupported(who, "too many query rows");
+  // (a grid holds less than 2^32 threads along x)
+  if (tiles * c.nkv >= 1ull << 24) return unsupported(who, "2^29 or more query columns");
   p->tiles = (uint32_t)tiles;
   if (p->rows) return GH_OK;
   uint64_t tokens = (uint64_t)r.max_pages << c.page_shift;

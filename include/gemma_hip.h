@@ -302,7 +302,8 @@ gh_status gh_prefill_gate_up_geglu(gh_context *ctx, gh_quant_mode mode, const vo
  *   *_scale f32  [num_pages][num_kv][blocks]
  * with blocks = page_tokens / 16; v's element (token 4 a + b, dim d) of a block
  * lies at [a][d][b].  page_tokens is 16, 32, 64, 128 or 256; head_dim a
- * multiple of 16 up to 512; k and v 16-byte aligned.  Fresh memory needs no
+ * multiple of 16 up to 512, num_kv at most 4096, and the blocks of all pages
+ * and heads fewer than 2^32; k and v 16-byte aligned.  Fresh memory needs no
  * clearing. */
 #define GH_KV8_BLOCK 16
 typedef struct gh_kv8_cache {
@@ -322,7 +323,8 @@ size_t gh_kv8_scale_bytes(const gh_kv8_cache *cache);
  * token past the table's end, or whose entry is not below num_pages, has no
  * page: it is not kept, reads as 0 and is attended to by no one.  Sequences may
  * share pages that are read; a page that a call appends to must be named once.
- * Rows of arguments that belong to no sequence are not touched. */
+ * Rows of arguments that belong to no sequence are not touched.  At most 65535
+ * sequences, 1000000 rows and 65536 query heads a call. */
 typedef struct gh_kv8_batch {
   const uint32_t *seq_start, *past, *pages;
   uint32_t num_seqs, max_pages, num_rows, max_rows;
@@ -358,7 +360,8 @@ gh_status gh_kv8_read(gh_context *ctx, const gh_kv8_cache *cache, const gh_kv8_b
  * tokens t of its sequence with t <= its own and, when window > 0, t > its own -
  * window, of scale * (Q . K[t]), times V[t]; query head h reads kv head h /
  * (num_q / num_kv).  Q and out are [num_rows][num_q * head_dim], 16-byte
- * aligned.  A row that sees no token is 0.  The rows' own tokens must be in the
+ * aligned.  A row that sees no token is 0; a query head with a NaN or infinite
+ * element, or that sees a token whose block has a NaN scale, is NaN.  The rows' own tokens must be in the
  * cache (gh_kv8_append).  max_kv: about the most tokens of a sequence, its rows
  * included (0: what the table holds); it and the window set how the work is
  * split, not what is computed. */
@@ -371,7 +374,8 @@ gh_status gh_kv8_attn(gh_context *ctx, const gh_kv8_cache *cache, const gh_kv8_b
 /* probs = softmax(y / temperature) of each row, y = softcap * tanh(logit /
  * softcap), or the logit when softcap is 0; a logit of -inf is masked (0) either
  * way, and a row of them gives zeros; a row with a NaN (or, without a softcap, a
- * +inf) gives NaN.  Rows are stride floats apart in both; probs may be logits. */
+ * +inf) gives NaN.  Rows are stride floats apart in both; probs may be logits.
+ * At most 65535 rows. */
 size_t gh_logit_probs_workspace(const gh_context *ctx, uint32_t rows, uint32_t vocab);
 gh_status gh_logit_probs(gh_context *ctx, const float *logits, float *probs, uint32_t rows,
                          uint32_t vocab, uint32_t stride, float softcap, float temperature,
@@ -387,7 +391,7 @@ gh_status gh_logit_probs(gh_context *ctx, const float *logits, float *probs, uin
  * as 0.  out_tokens [num_seqs][max_draft + 1] gets the kept drafts, the drawn
  * token and GH_NO_TOKEN after it; accepted[s] the number kept.  Where no weight
  * is positive, or their sum is infinite, the drawn token is GH_NO_TOKEN.  Sums
- * are in 64 bits. */
+ * are in 64 bits.  At most 65535 sequences and drafts of one, vocab below 2^31. */
 #define GH_NO_TOKEN 0xffffffffu
 size_t gh_spec_verify_workspace(const gh_context *ctx, uint32_t num_seqs, uint32_t vocab);
 gh_status gh_spec_verify(gh_context *ctx, const float *target, const float *draft,

@@ -1,6 +1,6 @@
 // serving.cpp -- the batched serving calls on a HIP runtime without a device: each line
-// read from stdin changes one argument of a call that is right ("name value"; "-" changes
-// nothing) and gives the status, and the kernels that are launched.
+// read from stdin changes arguments of a call that is right ("name value", or "a+b 1+2" for
+// two) and gives the status, and the kernels that are launched.
 //   serving DIR append|read|attn|probs|verify
 #include <math.h>
 #include <stdio.h>
@@ -20,8 +20,8 @@ int main(int argc, char** argv) {
   gh_context* made = nullptr;
   if (argc < 3 || gh_context_init(argv[1], &made) != GH_OK) return 2;
   const std::string call = argv[2];
-  char name[32], value[32];
-  while (scanf("%31s %31s", name, value) == 2) {
+  char name[96], value[96];
+  while (scanf("%95s %95s", name, value) == 2) {
     // (no kernel runs: the addresses only have the right alignment)
     std::map<std::string, double> v = {
         {"ctx", 1}, {"cache", 1}, {"batch", 1}, {"k", 4096}, {"v", 4096}, {"k_scale", 4096}, {"v_scale", 4096},
@@ -31,9 +31,14 @@ int main(int argc, char** argv) {
         {"rot", 64}, {"k_eq_v", 0}, {"theta", 10000}, {"eps", 1e-6}, {"scale", 1}, {"window", 0}, {"max_kv", 1000},
         {"work", 4096}, {"bytes", 1 << 30}, {"rows", 3}, {"vocab", 1000}, {"stride", 1000}, {"cap", 30}, {"temp", 1},
         {"draft", 4096}, {"tokens", 4096}, {"n_draft", 4096}, {"u", 4096}, {"pick", 4096}, {"accepted", 4096}, {"max_draft", 3}};
-    if (strcmp(name, "-") != 0) {
-      if (!v.count(name)) return 2;
-      v[name] = atof(value);
+    for (char *n = name, *x = value; n;) {
+      char *n2 = strchr(n, '+'), *x2 = n2 ? strchr(x, '+') : nullptr;
+      if (n2) *n2++ = 0;
+      if (x2) *x2++ = 0;
+      if (!v.count(n) || (n2 && !x2)) return 2;
+      v[n] = atof(x);
+      n = n2;
+      x = x2;
     }
     const auto at = [&](const char* n) { return reinterpret_cast<void*>((uintptr_t)v[n]); };
     const auto f = [&](const char* n) { return (float*)at(n); };

@@ -314,6 +314,21 @@ def test_attention_scales_far_apart_and_zero_blocks(gpu, run):
 
 
 @RUNS
+def test_attention_of_the_smallest_scales(gpu, run):
+    nq, H, D, page = 4, 2, 64, 16
+    rng = np.random.default_rng(19)
+    cache = ref.Cache(12, page, H, D, rng)
+    cache.scales[1][:] = 2.0 ** -126
+    dev = ref.Device(gpu, cache)
+    tables = np.arange(12, dtype=np.uint32)[None]
+    q = rng.standard_normal((2, nq, D)).astype(np.float32)
+    want, bound = ref.attention(cache, [2], [180], tables, q, 0.3, 0)
+    got = run(gpu, dev, [2], [180], tables, q, 0.3, 0)
+    # (sums below f32's normal range: half a step of 2^-149 a wave, a split and the quotient, 12 at most)
+    assert np.all(np.abs(got - want) <= bound + 6 * 2.0 ** -149)
+
+
+@RUNS
 def test_attention_masked_places_may_hold_anything(gpu, run):
     # NaN, infinite and huge scales behind a sequence's last token, in front of its window and in
     # pages of others change nothing; pages that are absent are as masked
@@ -492,3 +507,58 @@ def test_serving_loop(gpu):
         else:
             past = [x + r for x, r in zip(past, rows)]
         rows = [n + 1] * seqs
+
+
+def test_captured_step_with_sequences_that_grow(gpu):
+    """One recorded step (append, attention, probabilities, verification), replayed while the lengths,
+    rows and numbers in its arrays change, against the same calls made directly on a second cache."""
+    nq, H, D, page, V, n, seqs = 4, 2, 64, 16, 301, 2, 3
+    rng = np.random.default_rng(43)
+    T = seqs * (n + 1)
+    tables = tables_of(rng, seqs, 4, 12)
+    w = (nq + 2 * H) * D
+    sides = []
+    for _ in range(2):
+        dev = ref.Device(gpu, ref.Cache(12, page, H, D))
+        b = dev.batch([n + 1] * seqs, [0] * seqs, tables)
+        B = dict(dev=dev, b=b, X=gpu.alloc(T * w * 4), N=gpu.upload(np.ones(D, np.float32)), Q=gpu.alloc(T * nq * D * 4),
+                 O=gpu.alloc(T * nq * D * 4), L=gpu.alloc(T * V * 4), P=gpu.alloc(T * V * 4), K=gpu.alloc(seqs * n * 4),
+                 ND=gpu.alloc(seqs * 4), U=gpu.alloc(seqs * n * 4), I=gpu.alloc(seqs * 4), T=gpu.alloc(T * 4), A=gpu.alloc(seqs * 4))
+        B["sizes"] = sizes = (gpu.kv8_attn_workspace(dev.cache, b, nq, 0, 4 * page), gpu.logit_probs_workspace(T, V),
+                              gpu.spec_verify_workspace(seqs, V))
+        B["W"] = [gpu.alloc(max(x, 16)) for x in sizes]
+        sides.append(B)
+
+    def step(B):
+        gpu.kv8_append(B["dev"].cache, B["b"], B["X"].ptr, B["X"].ptr + 4 * nq * D, B["X"].ptr + 4 * (nq + H) * D, w, w,
+                       B["N"], B["N"], B["Q"], nq, D, False, 10000.0, EPS)
+        gpu.kv8_attn(B["dev"].cache, B["b"], B["Q"], B["O"], nq, 0.125, 0, 4 * page, B["W"][0], B["sizes"][0])
+        gpu.logit_probs(B["L"], B["P"], T, V, V, 30.0, 1.0, B["W"][1], B["sizes"][1])
+        gpu.spec_verify(B["P"], None, B["K"], B["ND"], B["U"], B["I"], B["T"], B["A"], seqs, n, V, B["W"][2], B["sizes"][2])
+
+    gpu.graph_begin()
+    step(sides[0])
+    graph = gpu.graph_end()
+    past = np.array([0, 5, 14], np.uint32)
+    for turn in range(5):
+        x = rng.standard_normal((T, w)).astype(np.float32)
+        logits = rng.standard_normal((T, V)).astype(np.float32) * 4
+        tokens, drafts = rng.integers(0, V, (seqs, n)).astype(np.uint32), rng.integers(0, n + 1, seqs).astype(np.uint32)
+        u, pick = rng.random((seqs, n), np.float32) * 0.1, rng.random(seqs, np.float32)
+        for B in sides:
+            for name, a in (("X", x), ("L", logits), ("K", tokens), ("ND", drafts), ("U", u), ("I", pick)):
+                B[name].write(a)
+            B["b"].held[1].write(past)
+        gpu.graph_launch(graph)
+        step(sides[1])
+        gpu.sync()
+        for name in ("Q", "O", "P", "T", "A"):
+            one, two = (B[name].read(np.uint32) for B in sides)
+            assert np.array_equal(one, two), (turn, name)
+        for one, two in zip(*(B["dev"].codes() + B["dev"].scales() for B in sides)):
+            assert np.array_equal(one, two)
+        past += 1 + sides[0]["A"].read(np.uint32)
+        for B in sides:  # nothing is left over from one turn for the next
+            for name in ("O", "P", "T"):
+                gpu.fill_u32(B[name], 0x7fc00000, B[name].nbytes // 4)
+    gpu.graph_destroy(graph)

@@ -40,7 +40,9 @@ def serving(tmp_path_factory):
 
 
 CACHE = [("ctx", 0, INVALID), ("cache", 0, INVALID), ("batch", 0, INVALID), ("k", 0, INVALID), ("v_scale", 0, INVALID),
-         ("k", 4104, INVALID), ("num_pages", 0, INVALID), ("num_pages", 4294967295, UNSUPPORTED), ("page_tokens", 8, UNSUPPORTED),
+         ("k", 4104, INVALID), ("num_pages", 0, INVALID), ("num_pages", 4294967295, UNSUPPORTED),
+         ("num_pages", 1073741824, UNSUPPORTED),  # 2^32 blocks
+         ("page_tokens", 8, UNSUPPORTED),
          ("page_tokens", 48, UNSUPPORTED), ("page_tokens", 512, UNSUPPORTED), ("head_dim", 0, INVALID), ("head_dim", 72, UNSUPPORTED),
          ("head_dim", 528, UNSUPPORTED), ("num_kv", 0, INVALID), ("seq_start", 0, INVALID), ("pages", 0, INVALID),
          ("past", 4098, INVALID), ("max_pages", 0, INVALID), ("num_seqs", 65536, UNSUPPORTED), ("num_rows", 1000001, UNSUPPORTED)]
@@ -52,9 +54,10 @@ REFUSED = {
     "read": CACHE + [("kin", 4097, INVALID)],
     "attn": CACHE + [("q", 0, INVALID), ("out", 0, INVALID), ("q", 4100, INVALID), ("num_q", 0, INVALID), ("num_q", 5, INVALID),
                      ("num_q", 65538, UNSUPPORTED), ("scale", "nan", INVALID), ("scale", "inf", INVALID), ("work", 0, INVALID), ("work", 4104, INVALID),
-                     ("bytes", 1, INVALID)],
+                     ("bytes", 1, INVALID),
+                     ("num_rows+max_rows+num_q", "1000000+1000000+65536", UNSUPPORTED)],
     "probs": [("ctx", 0, INVALID), ("q", 0, INVALID), ("out", 0, INVALID), ("out", 4097, INVALID), ("stride", 999, INVALID),
-              ("cap", -1, INVALID), ("cap", "nan", INVALID), ("temp", 0, INVALID), ("temp", -1, INVALID), ("temp", "nan", INVALID),
+              ("cap", -1, INVALID), ("cap", "nan", INVALID), ("cap", 1e-39, INVALID), ("temp", 0, INVALID), ("temp", -1, INVALID), ("temp", "nan", INVALID),
               ("temp", 1e-39, INVALID), ("rows", 65536, UNSUPPORTED), ("work", 0, INVALID), ("bytes", 1, INVALID)],
     "verify": [("ctx", 0, INVALID), ("q", 0, INVALID), ("tokens", 0, INVALID), ("u", 0, INVALID), ("pick", 0, INVALID), ("out", 0, INVALID),
                ("accepted", 0, INVALID), ("vocab", 0, INVALID), ("vocab", 2147483648, UNSUPPORTED), ("num_seqs", 65536, UNSUPPORTED),
