@@ -1129,6 +1129,10 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, 
   const uint64_t row = KV8_COLS * (uint64_t)(D + KV8_PART);
   const float* p = a.part + unit * a.nsplit * row + n * (uint64_t)(D + KV8_PART);
   __shared__ float f[KV8_MAX_SPLIT], red[8];
+  constexpr uint32_t N = 8;  // sums on their way at a time, the first of them before the factors
+  float x[N];
+#pragma unroll
+  for (uint32_t i = 0; i < N; i++) x[i] = i < live && tid < D ? p[i * row + tid] : 0.f;
   float m = -INFINITY, l = 0.f;
   if (tid < live) {
     m = p[tid * row + D];
@@ -1150,15 +1154,14 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, 
   float* out = a.out + row_at(a, t, t.col0 + n);
   for (uint32_t d = tid; d < D; d += 256) {
     float o = 0.f;
-    uint32_t s = 0;
-    for (; s + 8 <= live; s += 8) {
-      float x[8];
+    for (uint32_t s = 0; s < live; s += N) {
+      if (s > 0 || d >= 256) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = p[(s + i) * row + d];
+        for (uint32_t i = 0; i < N; i++) x[i] = s + i < live ? p[(s + i) * row + d] : 0.f;
+      }
 #pragma unroll
-      for (int i = 0; i < 8; i++) o = fmaf(x[i], f[s + i], o);
+      for (uint32_t i = 0; i < N; i++) o = fmaf(x[i], s + i < live ? f[s + i] : 0.f, o);
     }
-    for (; s < live; s++) o = fmaf(p[s * row + d], f[s], o);
     out[d] = o * by;
   }
 }
