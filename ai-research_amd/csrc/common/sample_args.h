@@ -14,7 +14,7 @@ struct ProbsArgs {
   float* part;  // [row][chunk] {max, sum}
   uint64_t stride;
   uint32_t vocab, chunks;
-  float cap, inv_cap, mul;  // soft-cap (0: none); log2(e) / temperature
+  float inv_cap, mul;  // 1 / soft-cap (0: none); log2(e) / temperature, times the soft-cap
 };
 
 struct VerifyArgs {

@@ -62,50 +62,55 @@ __device__ __forceinline__ float tanh_high(float y) {
   const float e = __builtin_amdgcn_exp2f(fabsf(y) * 2.885390082f);
   return copysignf(fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f), y);
 }
-// A thread's logits soft-capped.  Most rows have nothing past 0.7 cap: a wave
-// without takes the first form alone.
+// A thread's logits soft-capped, in units of the cap.  Most rows have nothing past 0.7
+// cap: a wave without takes the first form alone.
 template <uint32_t N>
-__device__ __forceinline__ void soft_cap(float (&x)[N], float cap, float inv_cap) {
-  if (!(cap > 0.f)) return;
-  bool far = false;
+__device__ __forceinline__ void soft_cap(float (&x)[N], float inv_cap) {
+  if (!(inv_cap > 0.f)) return;
+  float y[N], far = 0.f;
 #pragma unroll
-  for (uint32_t i = 0; i < N; i++) far |= !(fabsf(x[i] * inv_cap) < 0.7f);
-  if (__any(far)) {
+  for (uint32_t i = 0; i < N; i++) {
+    y[i] = x[i] * inv_cap;
+    far = fmaxf(far, fabsf(y[i]));
+  }
+  if (__any(!(far < 0.7f))) {
 #pragma unroll
-    for (uint32_t i = 0; i < N; i++) {
-      const float y = x[i] * inv_cap;
-      if (x[i] != -INFINITY) x[i] = cap * (fabsf(y) < 0.7f ? tanh_low(y) : tanh_high(y));
-    }
+    for (uint32_t i = 0; i < N; i++)
+      if (x[i] != -INFINITY) x[i] = fabsf(y[i]) < 0.7f ? tanh_low(y[i]) : tanh_high(y[i]);
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < N; i++) x[i] = cap * tanh_low(x[i] * inv_cap);
+    for (uint32_t i = 0; i < N; i++) x[i] = tanh_low(y[i]);
   }
 }
 
-// the workgroup's maximum and the sum relative to it, in every thread
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+// what is subtracted for a maximum (of nothing: 0)
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+// The workgroup's maximum and the sum relative to it, in every thread, from its waves'
+// maxima and their threads' sums relative to them.
 __device__ __forceinline__ void join(float* m, float* l, float mul) {
   __shared__ float sm[4], sl[4];
-  float M = *m, L = *l;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const float m2 = __shfl_xor(M, off, 64), l2 = __shfl_xor(L, off, 64), mx = fmaxf(M, m2);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    // in the order of the lanes, so that both of a pair get the same sum
-    const float a = L * __builtin_amdgcn_exp2f((M - base) * mul), b = l2 * __builtin_amdgcn_exp2f((m2 - base) * mul);
-    L = a + b;
-    M = mx;
-  }
   const uint32_t wave = threadIdx.x >> 6;
+  const float sum = wave_sum(*l);
   if ((threadIdx.x & 63) == 0) {
-    sm[wave] = M;
-    sl[wave] = L;
+    sm[wave] = *m;
+    sl[wave] = sum;
   }
   __syncthreads();
-  M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  const float base = M == -INFINITY ? 0.f : M;
-  L = 0.f;
+  const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  float L = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; w++) L += sl[w] * __builtin_amdgcn_exp2f((sm[w] - base) * mul);
+  for (int w = 0; w < 4; w++) L += sl[w] * __builtin_amdgcn_exp2f((sm[w] - base_of(M)) * mul);
   *m = M;
   *l = L;
 }
@@ -115,10 +120,11 @@ template <bool VEC, uint32_t N>
 __device__ __forceinline__ void probs_part(const ProbsArgs& a) {
   float x[N], m = -INFINITY, l = 0.f;
   load_chunk<VEC, N>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
-  soft_cap<N>(x, a.cap, a.inv_cap);
+  soft_cap<N>(x, a.inv_cap);
 #pragma unroll
   for (uint32_t i = 0; i < N; i++) m = fmaxf(m, x[i]);
-  const float base = m == -INFINITY ? 0.f : m;
+  m = wave_max(m);
+  const float base = base_of(m);
 #pragma unroll
   for (uint32_t i = 0; i < N; i++) l += __builtin_amdgcn_exp2f((x[i] - base) * a.mul);
   join(&m, &l, a.mul);
@@ -135,13 +141,16 @@ __device__ __forceinline__ void probs_write(const ProbsArgs& a) {
   load_chunk<VEC, N>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
   const float* p = a.part + 2 * (uint64_t)blockIdx.y * a.chunks;
   for (uint32_t c = threadIdx.x; c < a.chunks; c += 256) {
-    const float m2 = p[2 * c], l2 = p[2 * c + 1], mx = fmaxf(m, m2), base = mx == -INFINITY ? 0.f : mx;
+    const float m2 = p[2 * c], l2 = p[2 * c + 1], mx = fmaxf(m, m2), base = base_of(mx);
     l = l * __builtin_amdgcn_exp2f((m - base) * a.mul) + l2 * __builtin_amdgcn_exp2f((m2 - base) * a.mul);
     m = mx;
   }
-  soft_cap<N>(x, a.cap, a.inv_cap);
+  soft_cap<N>(x, a.inv_cap);
+  const float wm = wave_max(m);
+  l *= __builtin_amdgcn_exp2f((m - base_of(wm)) * a.mul);
+  m = wm;
   join(&m, &l, a.mul);
-  const float base = m == -INFINITY ? 0.f : m;
+  const float base = base_of(m);
   const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;  // every logit -inf: all 0
   const uint32_t start = blockIdx.x * (256 * N), left = a.vocab - start;
   float* out = a.probs + blockIdx.y * a.stride + start;

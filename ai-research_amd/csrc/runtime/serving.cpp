@@ -314,9 +314,10 @@ gh_status gh_logit_probs(gh_context* ctx, const float* logits, float* probs, uin
     gh_status st = check_work(who, work, work_bytes, gh_logit_probs_workspace(ctx, rows, vocab));
     if (st != GH_OK) return st;
     const uint32_t each = sample_each(ctx, rows, vocab);
-    ProbsArgs a{logits, probs, static_cast<float*>(work), stride, vocab, chunks_of(vocab, each), softcap,
-                softcap > 0.f ? 1.f / softcap : 0.f, (float)(1.4426950408889634 / (double)temperature)};
-    if (!(a.mul < INFINITY)) return invalid(who, "temperature is too small");
+    const double mul = 1.4426950408889634 / (double)temperature * (softcap > 0.f ? (double)softcap : 1.0);
+    ProbsArgs a{logits, probs, static_cast<float*>(work), stride, vocab, chunks_of(vocab, each),
+                softcap > 0.f ? 1.f / softcap : 0.f, (float)mul};
+    if (!(a.mul < INFINITY)) return invalid(who, "softcap / temperature is too large");
     if (!(a.inv_cap < INFINITY)) return invalid(who, "softcap is too small");
     const bool vec = vocab % 4 == 0 && stride % 4 == 0 && aligned(logits, 16) && aligned(probs, 16);
     void* args[] = {&a};

@@ -42,7 +42,7 @@ def test_probabilities_rows_in_a_wider_matrix(gpu):
         assert np.all(got[:2, vocab:] == 3.0)  # what lies between the rows
 
 
-@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("cap", [0.0, 30.0, 0.5])
 def test_probabilities_of_masked_and_broken_rows(gpu, cap):
     rng = np.random.default_rng(2)
     x = rng.standard_normal((6, 9001)).astype(np.float32)
