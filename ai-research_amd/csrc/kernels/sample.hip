@@ -42,7 +42,7 @@ __device__ __forceinline__ void load_chunk(const float* row, uint32_t c, uint32_
 // Probabilities: y = cap tanh(x / cap) (x without a cap; -inf stays), p =
 // 2^((y - max) log2(e) / temperature) / sum.  The first launch leaves each chunk's
 // maximum and sum, the second joins a row's and writes; it finds the logits in
-// the last-level cache.
+// the last-level cache.  (40 rows of 262144: 9.4 and 12.7 us, 4.5 and 6.6 TB/s.)
 // ---------------------------------------------------------------------------
 // tanh within 5 half steps, without the library's branches, which bounded the
 // kernels (40 rows of 262144: 17 us a launch at 2.5 TB/s): below 0.7 y + y^3 P(y^2),
@@ -172,7 +172,8 @@ __device__ __forceinline__ void probs_write(const ProbsArgs& a) {
 // Verification.  Draft i is kept while u_i q_i(x_i) < p_i(x_i) (exact in 64 bits);
 // where it stops, the token is drawn from what the target has over the draft,
 // max(p - q, 0), or from the target itself after the last draft.  A token is
-// decided next to a border, so weights and sums are in 64 bits.
+// decided next to a border, so weights and sums are in 64 bits.  (32 sequences of 262144:
+// 12.9 us for the chunks' sums, 5.2 TB/s, and 5.2 for the token, a chain of loads.)
 // ---------------------------------------------------------------------------
 struct Stop {
   uint32_t kept, drafts;

@@ -104,10 +104,10 @@ struct AttnPlan {
 // The other one splits the tokens where that shortens the whole: its four waves take
 // steps of 32 tokens in turn, 2.3 us for a step each (256 dims; 0.6 more of that for
 // every workgroup a CU has beyond one), and the splits' sums cost a launch and their
-// way through memory, 4 us and 3 TB/s.  (One token over 544, 8 heads: 5 splits 12 us,
-// none 19; 8 sequences of 32 rows over 2000, 256 tiles: none 45, 2 58; a prompt of 256
-// tokens, 256 tiles: none 11, 2 22; 32 sequences of 20 - 4000 tokens, 256 tiles: 2 67,
-// none 76.)  Parts are of equal length in tokens, so that long sequences of a batch
+// way through memory, 4 us and 3 TB/s.  (One token over 544, 8 heads: 5 splits 10.9 us,
+// none 13.7; 8 sequences of 32 rows over 2000, 256 tiles: none 45, 2 58; a prompt of 256
+// tokens, 256 tiles: none 11, 2 22; 32 sequences of 20 - 4000 tokens, 256 tiles: 2 66,
+// none 78; 8 of 5 rows over 1000 - 3000, 64 tiles: 6 24, none 49.)  Parts are of equal length in tokens, so that long sequences of a batch
 // take more of them than short ones, and at most as many as two a CU.
 gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, const Kv8Rows& r, uint32_t num_q,
                     uint32_t window, uint32_t max_kv, AttnPlan* p) {
