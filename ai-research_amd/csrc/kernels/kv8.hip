@@ -484,7 +484,8 @@ __device__ __forceinline__ uint32_t piece_at(uint32_t l, uint32_t D) {
   return FULL || 64 * l + 4 * n < D ? g * 4 * D + l * 256 + n * 16 : 0;
 }
 
-template <int NL, bool FULL, bool IS_K>
+// STREAM: nothing is read again, and the codes pass by the caches.
+template <int NL, bool FULL, bool STREAM, bool IS_K>
 __device__ __forceinline__ void load_codes(const Kv8AttnArgs& a, const Tile& t, uint32_t step, uint32_t pages, uint32_t i,
                                            Codes<NL>* s) {
   const uint32_t D = FULL ? 64 * NL : a.c.D;
@@ -497,7 +498,10 @@ __device__ __forceinline__ void load_codes(const Kv8AttnArgs& a, const Tile& t, 
     s->s[b] = (IS_K ? a.c.ks : a.c.vs)[at];
     const int8_t* c = (IS_K ? a.c.k : a.c.v) + (uint64_t)at * (KV8_BLOCK * D);
 #pragma unroll
-    for (int l = 0; l < NL; l++) s->c[b][l] = *reinterpret_cast<const i32x4*>(c + piece_at<FULL, IS_K>(l, D));
+    for (int l = 0; l < NL; l++) {
+      const i32x4* p = reinterpret_cast<const i32x4*>(c + piece_at<FULL, IS_K>(l, D));
+      s->c[b][l] = STREAM ? __builtin_nontemporal_load(p) : *p;
+    }
   }
 }
 
@@ -827,7 +831,7 @@ __device__ __forceinline__ void write_dims(const f32x4 (&o)[4], float* to, uint3
 // digits are in LDS to leave the registers to them.  (Heads of 256 over 8 key heads: 32
 // rows over 20 - 4000 tokens 62 us, 4.3 TB/s of codes; one row over 120000 91 us, 5.4.)
 // grid (tiles * splits, kv heads, sequences)
-template <int NL, bool FULL>
+template <int NL, bool FULL, bool STREAM>
 __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   extern __shared__ __align__(16) char lds[];
   const uint32_t lane = threadIdx.x & 63, wave = wave_id(), n = lane & 15, g = lane >> 4;
@@ -853,8 +857,8 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   Codes<NL> k, v;
   uint32_t i = 0, s = s0 + wave;
   if (s < s1) {
-    load_codes<NL, FULL, true>(a, t, s, pages, 0, &k);
-    load_codes<NL, FULL, false>(a, t, s, pages, 0, &v);
+    load_codes<NL, FULL, STREAM, true>(a, t, s, pages, 0, &k);
+    load_codes<NL, FULL, STREAM, false>(a, t, s, pages, 0, &v);
   }
   const float qmul = stage_q<NL>(row, lm, qd) * (a.scale * kLog2e);
   Run<NL> r;
@@ -867,12 +871,12 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
       i = 0;
       pages = step_pages(a, t, s + 4, 4);
     }
-    if (more) load_codes<NL, FULL, true>(a, t, s + 4, pages, i, &k);
+    if (more) load_codes<NL, FULL, STREAM, true>(a, t, s + 4, pages, i, &k);
     __builtin_amdgcn_sched_barrier(0);
     f16x8 hi, lo;
     soft_step<NL, 0>(sc, v.s, v.has, &r, &hi, &lo);
     value_step<NL>(v, hi, lo, &r);
-    if (more) load_codes<NL, FULL, false>(a, t, s + 4, pages, i, &v);
+    if (more) load_codes<NL, FULL, STREAM, false>(a, t, s + 4, pages, i, &v);
     __builtin_amdgcn_sched_barrier(0);
   }
   r.l += __shfl_xor(r.l, 16, 64);
@@ -1110,8 +1114,10 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_append_p2_k(Kv8AppendAr
 extern "C" __global__ __launch_bounds__(256) void gh_kv8_append_p4_k(Kv8AppendArgs a) { append<4>(a); }
 
 #define KV8_ATTN(NL, WAVES)                                                                                       \
-  extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_attn_l##NL##_k(Kv8AttnArgs a) { attend<NL, true>(a); } \
-  extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_attn_l##NL##r_k(Kv8AttnArgs a) { attend<NL, false>(a); } \
+  extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_attn_l##NL##_k(Kv8AttnArgs a) { attend<NL, true, false>(a); } \
+  extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_attn_l##NL##r_k(Kv8AttnArgs a) { attend<NL, false, false>(a); } \
+  extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_attn_l##NL##s_k(Kv8AttnArgs a) { attend<NL, true, true>(a); } \
+  extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_attn_l##NL##rs_k(Kv8AttnArgs a) { attend<NL, false, true>(a); } \
   extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_rows_l##NL##_k(Kv8AttnArgs a) { attend_rows<NL, true>(a); } \
   extern "C" __global__ __launch_bounds__(256, WAVES) void gh_kv8_rows_l##NL##r_k(Kv8AttnArgs a) { attend_rows<NL, false>(a); }
 KV8_ATTN(1, 2)

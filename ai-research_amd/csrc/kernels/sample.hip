@@ -13,12 +13,13 @@
 namespace {
 
 // A thread's elements of chunk c: VEC: float4, 1 KB apart in a wave's row; else
-// single floats.  Elements past the row are `none`.
+// single floats.  Elements past the row are `none`.  STREAM: they are not read again,
+// and pass by the caches.
 template <bool VEC>
 __device__ __forceinline__ uint32_t elem(uint32_t i) {
   return VEC ? (i >> 2) * 1024 + threadIdx.x * 4 + (i & 3) : i * 256 + threadIdx.x;
 }
-template <bool VEC, uint32_t N>
+template <bool VEC, uint32_t N, bool STREAM>
 __device__ __forceinline__ void load_chunk(const float* row, uint32_t c, uint32_t vocab, float none, float (&x)[N]) {
   const uint32_t base = c * (256 * N), left = vocab - base;
   row += base;
@@ -26,12 +27,12 @@ __device__ __forceinline__ void load_chunk(const float* row, uint32_t c, uint32_
   for (uint32_t i = 0; i < N; i += VEC ? 4 : 1) {
     const uint32_t e = elem<VEC>(i);
     if (VEC) {  // (vocab is a multiple of 4 there)
-      float4 v = {none, none, none, none};
-      if (e < left) v = *reinterpret_cast<const float4*>(row + e);
-      x[i] = v.x;
-      x[i + 1] = v.y;
-      x[i + 2] = v.z;
-      x[i + 3] = v.w;
+      typedef float f32x4 __attribute__((ext_vector_type(4)));
+      f32x4 v = {none, none, none, none};
+      const f32x4* p = reinterpret_cast<const f32x4*>(row + e);
+      if (e < left) v = STREAM ? __builtin_nontemporal_load(p) : *p;
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) x[i + j] = v[j];
     } else {
       x[i] = e < left ? row[e] : none;
     }
@@ -119,7 +120,7 @@ __device__ __forceinline__ void join(float* m, float* l, float mul) {
 template <bool VEC, uint32_t N>
 __device__ __forceinline__ void probs_part(const ProbsArgs& a) {
   float x[N], m = -INFINITY, l = 0.f;
-  load_chunk<VEC, N>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
+  load_chunk<VEC, N, false>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
   soft_cap<N>(x, a.inv_cap);
 #pragma unroll
   for (uint32_t i = 0; i < N; i++) m = fmaxf(m, x[i]);
@@ -138,7 +139,7 @@ __device__ __forceinline__ void probs_part(const ProbsArgs& a) {
 template <bool VEC, uint32_t N>
 __device__ __forceinline__ void probs_write(const ProbsArgs& a) {
   float x[N], m = -INFINITY, l = 0.f;
-  load_chunk<VEC, N>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
+  load_chunk<VEC, N, false>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
   const float* p = a.part + 2 * (uint64_t)blockIdx.y * a.chunks;
   for (uint32_t c = threadIdx.x; c < a.chunks; c += 256) {
     const float m2 = p[2 * c], l2 = p[2 * c + 1], mx = fmaxf(m, m2), base = base_of(mx);
@@ -238,9 +239,9 @@ __device__ __forceinline__ void verify_part(const VerifyArgs& a) {
   const Stop s = stop_of(a, b);
   const Rows r = rows_of(a, b, s);
   float p[N], q[N];
-  load_chunk<VEC, N>(r.p, c, a.vocab, 0.f, p);
+  load_chunk<VEC, N, true>(r.p, c, a.vocab, 0.f, p);
   if (r.q) {
-    load_chunk<VEC, N>(r.q, c, a.vocab, 0.f, q);
+    load_chunk<VEC, N, true>(r.q, c, a.vocab, 0.f, q);
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < N; i++) q[i] = 0.f;

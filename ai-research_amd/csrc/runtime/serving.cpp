@@ -89,6 +89,7 @@ uint32_t dims64(const Kv8View& c) { return c.D <= 64 ? 1 : c.D <= 128 ? 2 : c.D 
 
 struct AttnPlan {
   bool rows = false;  // the kernel of many columns
+  bool stream = false;
   uint32_t tiles = 0, nsplit = 1, chunk = 1;
   size_t bytes = 0;
 };
@@ -109,6 +110,11 @@ struct AttnPlan {
 // tokens, 256 tiles: none 11, 2 22; 32 sequences of 20 - 4000 tokens, 256 tiles: 2 66,
 // none 78; 8 of 5 rows over 1000 - 3000, 64 tiles: 6 24, none 49.)  Parts are of equal length in tokens, so that long sequences of a batch
 // take more of them than short ones, and at most as many as two a CU.
+//
+// Codes that one tile reads once, and that are too many to be in the last-level cache
+// (256 MB) at the next call, pass by the caches: from 96 MB on, going by the bounds.  (One
+// row over 120000, 492 MB: 90 us by them and 102 through them; 16 sequences over 2000,
+// 131 MB: 30 and 34; 8 over 2000, 65 MB, the same three caches in turn: 21 and 20.)
 gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, const Kv8Rows& r, uint32_t num_q,
                     uint32_t window, uint32_t max_kv, AttnPlan* p) {
   if (num_q == 0 || num_q % c.nkv) return invalid(who, "num_q must be a positive multiple of the kv heads");
@@ -140,6 +146,7 @@ gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, co
     }
   }
   p->chunk = (uint32_t)((steps + p->nsplit - 1) / p->nsplit);
+  p->stream = tiles == 1 && units * steps >= (96ull << 20) / (2 * KV8_STEP * c.D);
   if (p->nsplit > 1) p->bytes = (size_t)units * p->nsplit * KV8_COLS * (c.D + KV8_PART) * sizeof(float);
   return GH_OK;
 }
@@ -282,9 +289,9 @@ gh_status gh_kv8_attn(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8_b
     a.chunk = p.chunk;
     a.scale = scale;
     const uint32_t nl = dims64(a.c);
-    // r: heads of fewer dims than the kernel's 64 nl
+    // r: heads of fewer dims than the kernel's 64 nl; s: codes by the caches
     const std::string name = std::string(p.rows ? "gh_kv8_rows_l" : "gh_kv8_attn_l") + std::to_string(nl) +
-                             (a.c.D == 64 * nl ? "_k" : "r_k");
+                             (a.c.D == 64 * nl ? "" : "r") + (p.stream ? "s_k" : "_k");
     void* args[] = {&a};
     if (p.rows) return launch(ctx, name.c_str(), dim3(p.tiles * a.c.nkv, 1, a.b.num_seqs), dim3(256), 14336 * nl, args);
     st = launch(ctx, name.c_str(), dim3(p.tiles * p.nsplit, a.c.nkv, a.b.num_seqs), dim3(256), 512 + 16384 * nl, args);
