@@ -829,7 +829,7 @@ __device__ __forceinline__ void write_dims(const f32x4 (&o)[4], float* to, uint3
 // tokens' bytes bound it, so a wave has the next step's keys on the way while it
 // weighs this step's values, and the next values while it scores; the query
 // digits are in LDS to leave the registers to them.  (Heads of 256 over 8 key heads: 32
-// rows over 20 - 4000 tokens 62 us, 4.3 TB/s of codes; one row over 120000 91 us, 5.4.)
+// rows over 20 - 4000 tokens 55 us, 4.8 TB/s of codes; one row over 120000 81 us, 6.1.)
 // grid (tiles * splits, kv heads, sequences)
 template <int NL, bool FULL, bool STREAM>
 __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
@@ -1176,10 +1176,11 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, 
 }
 
 namespace {
-// (wide: 16-byte aligned)
+// (wide: 16-byte aligned; by the caches: 2000 rows of 8 heads of 256 8.2 us, 5.0
+// TB/s; through them 9.0)
 __device__ __forceinline__ void write4(float* to, f32x4 x, uint32_t wide) {
   if (wide) {
-    *reinterpret_cast<f32x4*>(to) = x;
+    __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(to));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; i++) to[i] = x[i];
@@ -1188,8 +1189,7 @@ __device__ __forceinline__ void write4(float* to, f32x4 x, uint32_t wide) {
 }  // namespace
 
 // Read-back: the rows that a batch names as the values their codes stand for;
-// rows of places without a page are 0.  (2000 rows of 8 heads of 256: 9 us, 4.6 TB/s.)
-// grid (kv heads, blocks, sequences)
+// rows of places without a page are 0.  grid (kv heads, blocks, sequences)
 extern "C" __global__ __launch_bounds__(256) void gh_kv8_read_k(Kv8ReadArgs a) {
   const uint32_t seq = blockIdx.z, head = blockIdx.x, D = a.c.D;
   uint32_t first;

@@ -12,6 +12,8 @@
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 // A thread's elements of chunk c: VEC: float4, 1 KB apart in a wave's row; else
 // single floats.  Elements past the row are `none`.  STREAM: they are not read again,
 // and pass by the caches.
@@ -27,7 +29,6 @@ __device__ __forceinline__ void load_chunk(const float* row, uint32_t c, uint32_
   for (uint32_t i = 0; i < N; i += VEC ? 4 : 1) {
     const uint32_t e = elem<VEC>(i);
     if (VEC) {  // (vocab is a multiple of 4 there)
-      typedef float f32x4 __attribute__((ext_vector_type(4)));
       f32x4 v = {none, none, none, none};
       const f32x4* p = reinterpret_cast<const f32x4*>(row + e);
       if (e < left) v = STREAM ? __builtin_nontemporal_load(p) : *p;
@@ -43,7 +44,9 @@ __device__ __forceinline__ void load_chunk(const float* row, uint32_t c, uint32_
 // Probabilities: y = cap tanh(x / cap) (x without a cap; -inf stays), p =
 // 2^((y - max) log2(e) / temperature) / sum.  The first launch leaves each chunk's
 // maximum and sum, the second joins a row's and writes; it finds the logits in
-// the last-level cache.  (40 rows of 262144: 9.4 and 12.7 us, 4.5 and 6.6 TB/s.)
+// the last-level cache.  (40 rows of 262144: 20 us a call among others, 23 when the
+// second's loads and stores stay in the caches; 4 bytes read and 4 written an element
+// at the rate of a copy are 17.7.)
 // ---------------------------------------------------------------------------
 // tanh within 5 half steps, without the library's branches, which bounded the
 // kernels (40 rows of 262144: 17 us a launch at 2.5 TB/s): below 0.7 y + y^3 P(y^2),
@@ -139,7 +142,7 @@ __device__ __forceinline__ void probs_part(const ProbsArgs& a) {
 template <bool VEC, uint32_t N>
 __device__ __forceinline__ void probs_write(const ProbsArgs& a) {
   float x[N], m = -INFINITY, l = 0.f;
-  load_chunk<VEC, N, false>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
+  load_chunk<VEC, N, true>(a.logits + blockIdx.y * a.stride, blockIdx.x, a.vocab, -INFINITY, x);
   const float* p = a.part + 2 * (uint64_t)blockIdx.y * a.chunks;
   for (uint32_t c = threadIdx.x; c < a.chunks; c += 256) {
     const float m2 = p[2 * c], l2 = p[2 * c + 1], mx = fmaxf(m, m2), base = base_of(mx);
@@ -162,7 +165,7 @@ __device__ __forceinline__ void probs_write(const ProbsArgs& a) {
     const uint32_t e = elem<VEC>(i);
     if (e >= left) continue;
     if (VEC) {
-      *reinterpret_cast<float4*>(out + e) = float4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+      __builtin_nontemporal_store(f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]}, reinterpret_cast<f32x4*>(out + e));
     } else {
       out[e] = x[i];
     }
@@ -174,7 +177,7 @@ __device__ __forceinline__ void probs_write(const ProbsArgs& a) {
 // where it stops, the token is drawn from what the target has over the draft,
 // max(p - q, 0), or from the target itself after the last draft.  A token is
 // decided next to a border, so weights and sums are in 64 bits.  (32 sequences of 262144:
-// 12.9 us for the chunks' sums, 5.2 TB/s, and 5.2 for the token, a chain of loads.)
+// 12.6 us for the chunks' sums, 5.3 TB/s, and 5.2 for the token, a chain of loads.)
 // ---------------------------------------------------------------------------
 struct Stop {
   uint32_t kept, drafts;
