@@ -97,23 +97,28 @@ struct AttnPlan {
 // Which kernel, and into how many parts each sequence's tokens are split.
 //
 // The kernel of many columns halves what is read and converted a column, and wants many
-// workgroups: it is taken where tiles of 16 columns alone give every CU two of them.
+// workgroups: it is taken where several tiles of 16 columns a sequence alone give every CU
+// two of them.
 // (us with it and with the other one, 8 key heads of 256 under 16 query heads: prompts
 // of 2000 tokens 98 / 120, 700: 31 / 32, 8 of 64 rows over 1000: 41 / 47, over 4000: 123
-// / 158; with fewer tiles, a prompt of 500: 24 / 20, 8 of 32 over 2000: 47 / 45.)
+// / 158; with fewer tiles, a prompt of 500: 24 / 20, 8 of 32 over 2000: 47 / 45; with one
+// tile, 100 single rows over 500 - 3000: 177 / 135.)
 //
 // The other one splits the tokens where that shortens the whole: its four waves take
 // steps of 32 tokens in turn, 2.3 us for a step each (256 dims; 0.6 more of that for
-// every workgroup a CU has beyond one), and the splits' sums cost a launch and their
+// every workgroup that some CU has beyond one), and the splits' sums cost a launch and their
 // way through memory, 4 us and 3 TB/s.  (One token over 544, 8 heads: 5 splits 10.9 us,
 // none 13.7; 8 sequences of 32 rows over 2000, 256 tiles: none 45, 2 58; a prompt of 256
 // tokens, 256 tiles: none 11, 2 22; 32 sequences of 20 - 4000 tokens, 256 tiles: 2 66,
-// none 78; 8 of 5 rows over 1000 - 3000, 64 tiles: 6 24, none 49.)  Parts are of equal length in tokens, so that long sequences of a batch
-// take more of them than short ones, and at most as many as two a CU.
+// none 78; 8 of 5 rows over 1000 - 3000, 64 tiles: 6 24, none 49.)  Parts are of equal
+// length in tokens, so that long sequences of a batch take more of them than short ones.
+// They are at most as many as two workgroups a CU, which even out lengths that differ; one
+// a CU where there is one sequence and tile (one row over 120000 tokens: 85 us with one, 90
+// with two; over 30000: 31 and 33).
 //
 // Codes that one tile reads once, and that are too many to be in the last-level cache
 // (256 MB) at the next call, pass by the caches: from 96 MB on, going by the bounds.  (One
-// row over 120000, 492 MB: 90 us by them and 102 through them; 16 sequences over 2000,
+// row over 120000, 492 MB: 85 us by them and 94 through them; 16 sequences over 2000,
 // 131 MB: 30 and 34; 8 over 2000, 65 MB, the same three caches in turn: 21 and 20.)
 gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, const Kv8Rows& r, uint32_t num_q,
                     uint32_t window, uint32_t max_kv, AttnPlan* p) {
@@ -123,7 +128,7 @@ gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, co
   if (empty(r)) return GH_OK;
   const uint64_t G = num_q / c.nkv, cols = r.max_rows * G, cus = std::max(ctx->num_cus, 1);
   uint64_t tiles = (cols + KV8_COLS - 1) / KV8_COLS, units = tiles * c.nkv * r.num_seqs;
-  p->rows = units >= 2 * cus;
+  p->rows = tiles > 1 && units >= 2 * cus;
   if (p->rows) tiles = (cols + KV8_ROW_COLS - 1) / KV8_ROW_COLS;
   // (a grid holds less than 2^32 threads along x)
   if (tiles * c.nkv >= 1ull << 24) return unsupported(who, "2^29 or more query columns");
@@ -133,11 +138,12 @@ gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, co
   if (max_kv) tokens = std::min<uint64_t>(tokens, max_kv);
   if (window) tokens = std::min<uint64_t>(tokens, (uint64_t)window + (KV8_COLS + G - 1) / G);
   const uint64_t steps = tokens / KV8_STEP + 1;
-  const uint64_t most = std::min<uint64_t>({(steps + 3) / 4, 2 * cus / units, KV8_MAX_SPLIT});
+  const uint64_t a_cu = tiles == 1 && r.num_seqs == 1 ? 1 : 2;
+  const uint64_t most = std::min<uint64_t>({(steps + 3) / 4, a_cu * cus / units, KV8_MAX_SPLIT});
   double least = INFINITY;
   for (uint64_t n = 1; n <= std::max<uint64_t>(most, 1); n++) {
     const double turns = (double)(((steps + n - 1) / n + 3) / 4), each = 2.3 * std::max(0.5, c.D / 256.0);
-    const double load = std::max(1.0, 1 + 0.6 * ((double)(units * n) / (double)cus - 1));
+    const double load = 1 + 0.6 * (double)((units * n - 1) / cus);
     const double join = n > 1 ? 4 + (double)(units * n) * c.D * (2 * sizeof(float) * KV8_COLS) / 3e6 : 0;
     const double us = turns * each * load + join;
     if (us < least) {

@@ -259,7 +259,16 @@ def run_many(gpu, dev, rows, past, tables, q, scale, window, max_kv=0, **bounds)
     return got[:len(q)]
 
 
-RUNS = pytest.mark.parametrize("run", [run_attn, run_many])
+def run_stream(gpu, dev, rows, past, tables, q, scale, window, max_kv=0, **bounds):
+    """The same with tables that have room for 96 MB of codes: loads that pass by the caches."""
+    c = dev.c
+    tokens = (96 << 20) // (2 * c.D * c.H * len(rows)) + 64
+    wide = np.full((len(rows), max(tables.shape[1], tokens // c.page + 1)), 0xffffffff, np.uint32)
+    wide[:, :tables.shape[1]] = tables
+    return run_attn(gpu, dev, rows, past, wide, q, scale, window, max_kv, **bounds)
+
+
+RUNS = pytest.mark.parametrize("run", [run_attn, run_many, run_stream])
 ATTN = [  # nq, H, D, page, rows, past, window, scale
     (16, 8, 256, 16, [1], [543], 0, 1.0),
     (16, 8, 256, 32, [1, 1, 1, 1, 0, 1], [0, 15, 16, 700, 40, 129], 0, 0.0625),
@@ -276,6 +285,7 @@ ATTN = [  # nq, H, D, page, rows, past, window, scale
     (5, 1, 400, 32, [2, 30], [64, 1], 0, 0.05),
     (3, 1, 272, 16, [1], [0], 0, 0.06),
     (4, 4, 256, 16, [1], [2500], 0, 0.0625),
+    (8, 8, 64, 16, [1] * 70, [(37 * i) % 90 for i in range(70)], 0, 0.125),
 ]
 
 

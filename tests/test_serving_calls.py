@@ -90,6 +90,17 @@ def test_arguments_that_may_be_absent(serving):
         assert serving("verify", (name, 0))[0][0] == 0
 
 
+def test_kernels_by_sizes(serving):
+    # one tile; codes that may be 96 MB, in heads of 64 dims and of fewer; tiles for every CU
+    for names, values, kernel in (("max_rows", "1", "gh_kv8_attn_l1_k"), ("max_rows+max_kv+max_pages", "1+0+40000", "gh_kv8_attn_l1s_k"),
+                                  ("max_rows+max_kv+max_pages+head_dim+rot", "1+0+40000+48+0", "gh_kv8_attn_l1rs_k"),
+                                  ("head_dim", "96", "gh_kv8_attn_l2r_k"), ("head_dim", "512", "gh_kv8_attn_l8_k"),
+                                  ("num_rows+max_rows", "9000+9000", "gh_kv8_rows_l1_k"), ("num_seqs+max_rows", "300+1", "gh_kv8_attn_l1_k")):
+        (st, need, why, kernels), = serving("attn", (names, values))
+        assert st == 0 and kernels[0][0] == kernel, (names, why, kernels)
+        assert (need > 0) == (len(kernels) == 2)
+
+
 def test_grids_cover_the_rows(serving):
     # a sequence's rows can begin at a block's last token: 9 rows touch 2 blocks, 18 rows 3
     for rows, blocks in ((1, 1), (2, 2), (9, 2), (17, 2), (18, 3)):
