@@ -321,6 +321,8 @@ gh_status gh_logit_probs(gh_context* ctx, const float* logits, float* probs, uin
     if (!(softcap >= 0.f) || !(softcap < INFINITY)) return invalid(who, "softcap must be 0 (none) or positive");
     if (!(temperature > 0.f) || !(temperature < INFINITY)) return invalid(who, "temperature must be positive");
     if (rows > kMaxGrid) return unsupported(who, "more than 65535 rows");
+    // (the second launch's workgroups each join all chunks of their row)
+    if (vocab > 1u << 24) return unsupported(who, "vocab above 2^24");
     if (rows == 0 || vocab == 0) return GH_OK;
     if (!logits || !probs) return invalid(who, "logits or probs is null");
     if (!aligned(logits, 4) || !aligned(probs, 4)) return invalid(who, "rows must be 4-byte aligned");
@@ -360,6 +362,7 @@ gh_status gh_spec_verify(gh_context* ctx, const float* target, const float* draf
     if (num_seqs == 0) return GH_OK;
     if (!target || !pick || !out_tokens || !accepted || (max_draft && (!tokens || !u)))
       return invalid(who, "null pointer");
+    if (accepted == n_draft || out_tokens == tokens) return invalid(who, "accepted is n_draft, or out_tokens tokens");
     for (const void* p : {(const void*)target, (const void*)draft, (const void*)tokens, (const void*)n_draft,
                           (const void*)u, (const void*)pick, (const void*)out_tokens, (const void*)accepted})
       if (!aligned(p, 4)) return invalid(who, "arrays must be 4-byte aligned");

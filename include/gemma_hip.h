@@ -360,7 +360,7 @@ gh_status gh_kv8_read(gh_context *ctx, const gh_kv8_cache *cache, const gh_kv8_b
  * tokens t of its sequence with t <= its own and, when window > 0, t > its own -
  * window, of scale * (Q . K[t]), times V[t]; query head h reads kv head h /
  * (num_q / num_kv).  Q and out are [num_rows][num_q * head_dim], 16-byte
- * aligned.  A row that sees no token is 0; a query head with a NaN or infinite
+ * aligned, and may be the same.  A row that sees no token is 0; a query head with a NaN or infinite
  * element, or that sees a token whose block has a NaN scale, is NaN.  The rows' own tokens must be in the
  * cache (gh_kv8_append).  max_kv: about the most tokens of a sequence, its rows
  * included (0: what the table holds); it and the window set how the work is
@@ -375,7 +375,7 @@ gh_status gh_kv8_attn(gh_context *ctx, const gh_kv8_cache *cache, const gh_kv8_b
  * softcap), or the logit when softcap is 0; a logit of -inf is masked (0) either
  * way, and a row of them gives zeros; a row with a NaN (or, without a softcap, a
  * +inf) gives NaN.  Rows are stride floats apart in both; probs may be logits.
- * At most 65535 rows. */
+ * At most 65535 rows, vocab at most 2^24. */
 size_t gh_logit_probs_workspace(const gh_context *ctx, uint32_t rows, uint32_t vocab);
 gh_status gh_logit_probs(gh_context *ctx, const float *logits, float *probs, uint32_t rows,
                          uint32_t vocab, uint32_t stride, float softcap, float temperature,
@@ -391,7 +391,7 @@ gh_status gh_logit_probs(gh_context *ctx, const float *logits, float *probs, uin
  * as 0.  out_tokens [num_seqs][max_draft + 1] gets the kept drafts, the drawn
  * token and GH_NO_TOKEN after it; accepted[s] the number kept.  Where no weight
  * is positive, or their sum is infinite, the drawn token is GH_NO_TOKEN.  Sums
- * are in 64 bits.  At most 65535 sequences and drafts of one, vocab below 2^31. */
+ * are in 64 bits.  Outputs may not be inputs.  At most 65535 sequences and drafts of one, vocab below 2^31. */
 #define GH_NO_TOKEN 0xffffffffu
 size_t gh_spec_verify_workspace(const gh_context *ctx, uint32_t num_seqs, uint32_t vocab);
 gh_status gh_spec_verify(gh_context *ctx, const float *target, const float *draft,

@@ -27,10 +27,10 @@ int main(int argc, char** argv) {
         {"ctx", 1}, {"cache", 1}, {"batch", 1}, {"k", 4096}, {"v", 4096}, {"k_scale", 4096}, {"v_scale", 4096},
         {"num_pages", 10}, {"page_tokens", 32}, {"num_kv", 2}, {"head_dim", 64}, {"seq_start", 4096}, {"past", 4096},
         {"pages", 4096}, {"num_seqs", 3}, {"max_pages", 40}, {"num_rows", 20}, {"max_rows", 9}, {"q", 4096}, {"kin", 4096},
-        {"vin", 4096}, {"qn", 4096}, {"kn", 4096}, {"out", 4096}, {"q_stride", 512}, {"kv_stride", 512}, {"num_q", 4},
+        {"vin", 4096}, {"qn", 4096}, {"kn", 4096}, {"out", 12288}, {"q_stride", 512}, {"kv_stride", 512}, {"num_q", 4},
         {"rot", 64}, {"k_eq_v", 0}, {"theta", 10000}, {"eps", 1e-6}, {"scale", 1}, {"window", 0}, {"max_kv", 1000},
         {"work", 4096}, {"bytes", 1 << 30}, {"rows", 3}, {"vocab", 1000}, {"stride", 1000}, {"cap", 30}, {"temp", 1},
-        {"draft", 4096}, {"tokens", 4096}, {"n_draft", 4096}, {"u", 4096}, {"pick", 4096}, {"accepted", 4096}, {"max_draft", 3}};
+        {"draft", 4096}, {"tokens", 4096}, {"n_draft", 20480}, {"u", 4096}, {"pick", 4096}, {"accepted", 4096}, {"max_draft", 3}};
     for (char *n = name, *x = value; n;) {
       char *n2 = strchr(n, '+'), *x2 = n2 ? strchr(x, '+') : nullptr;
       if (n2) *n2++ = 0;

@@ -440,6 +440,23 @@ def test_attention_of_long_prompts(gpu, nq, H, D, page, rows, past, window, scal
         at += n
 
 
+@pytest.mark.parametrize("rows,past", [([1, 3], [700, 90]), ([1100], [0])])
+def test_attention_in_place(gpu, rows, past):
+    nq, H, D, page = 8, 8, 64, 32
+    rng = np.random.default_rng(8)
+    per = max(-(-(p + r) // page) for p, r in zip(past, rows))
+    cache = ref.Cache(len(rows) * per, page, H, D, rng)
+    dev = ref.Device(gpu, cache)
+    tables = tables_of(rng, len(rows), per, cache.P)
+    q = rng.standard_normal((sum(rows), nq, D)).astype(np.float32)
+    want = run_attn(gpu, dev, rows, past, tables, q, 0.125, 0)
+    b = dev.batch(rows, past, tables)
+    n = gpu.kv8_attn_workspace(dev.cache, b, nq, 0, 0)
+    X, W = gpu.upload(q), gpu.alloc(max(n, 16))
+    gpu.kv8_attn(dev.cache, b, X, X, nq, 0.125, 0, 0, W, n)
+    assert np.array_equal(X.read(np.float32).reshape(q.shape), want)
+
+
 def test_attention_repeats_and_replays(gpu):
     # the same bits every time, also from two graphs that share the workspace
     nq, H, D, page = 16, 8, 256, 32

@@ -58,10 +58,12 @@ REFUSED = {
                      ("num_rows+max_rows+num_q", "1000000+1000000+65536", UNSUPPORTED)],
     "probs": [("ctx", 0, INVALID), ("q", 0, INVALID), ("out", 0, INVALID), ("out", 4097, INVALID), ("stride", 999, INVALID),
               ("cap", -1, INVALID), ("cap", "nan", INVALID), ("cap", 1e-39, INVALID), ("temp", 0, INVALID), ("temp", -1, INVALID), ("temp", "nan", INVALID),
-              ("temp", 1e-39, INVALID), ("rows", 65536, UNSUPPORTED), ("work", 0, INVALID), ("bytes", 1, INVALID)],
+              ("temp", 1e-39, INVALID), ("rows", 65536, UNSUPPORTED),
+              ("vocab+stride", "16777217+16777217", UNSUPPORTED), ("work", 0, INVALID), ("bytes", 1, INVALID)],
     "verify": [("ctx", 0, INVALID), ("q", 0, INVALID), ("tokens", 0, INVALID), ("u", 0, INVALID), ("pick", 0, INVALID), ("out", 0, INVALID),
                ("accepted", 0, INVALID), ("vocab", 0, INVALID), ("vocab", 2147483648, UNSUPPORTED), ("num_seqs", 65536, UNSUPPORTED),
-               ("max_draft", 65536, UNSUPPORTED), ("draft", 4097, INVALID), ("work", 0, INVALID), ("bytes", 1, INVALID)],
+               ("max_draft", 65536, UNSUPPORTED), ("draft", 4097, INVALID),
+               ("accepted+n_draft", "8192+8192", INVALID), ("out+tokens", "8192+8192", INVALID), ("work", 0, INVALID), ("bytes", 1, INVALID)],
 }
 
 
