@@ -206,7 +206,8 @@ __device__ __forceinline__ void append_q(const Kv8AppendArgs& a, Angle* ang, uin
 #pragma unroll
       for (int m = 0; m < NP; m++) ss[j] += x0[j][m] * x0[j][m] + x1[j][m] * x1[j][m];
     }
-    const float root = 1.0f / sqrtf(wave_sums<R>(ss) / (float)D + a.eps);  // of row first + lane mod R
+    // of row first + lane mod R (once a row: in 64 bits, with one rounding)
+    const float root = (float)inverse_root((double)wave_sums<R>(ss) / (double)D + (double)a.eps);
 #pragma unroll
     for (int j = 0; j < R; j++) {
       const uint32_t r = first + j;
