@@ -830,7 +830,7 @@ __device__ __forceinline__ void write_dims(const f32x4 (&o)[4], float* to, uint3
 // tokens' bytes bound it, so a wave has the next step's keys on the way while it
 // weighs this step's values, and the next values while it scores; the query
 // digits are in LDS to leave the registers to them.  (Heads of 256 over 8 key heads: 32
-// rows over 20 - 4000 tokens 55 us, 4.8 TB/s of codes; one row over 120000 81 us, 6.1.)
+// rows over 20 - 4000 tokens 55 us, 4.8 TB/s of codes; one row over 120000 78 us, 6.3.)
 // grid (tiles * splits, kv heads, sequences)
 template <int NL, bool FULL, bool STREAM>
 __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
