@@ -82,7 +82,7 @@ def check_cache(cache, dev, tables, rows, past):
 
 SHAPES = [  # heads, kv heads, head dim, rotated dims, page
     (16, 8, 256, 256, 16), (16, 8, 256, 64, 64), (4, 4, 64, 32, 32), (12, 4, 96, 96, 128), (8, 1, 128, 0, 16),
-    (8, 2, 512, 128, 256), (3, 1, 16, 2, 16), (5, 1, 400, 400, 32), (2, 2, 272, 68, 16),
+    (8, 2, 512, 128, 256), (3, 1, 16, 2, 16), (5, 1, 400, 400, 32), (2, 2, 272, 68, 16), (2, 1, 512, 512, 32),
 ]
 
 
