@@ -9,7 +9,8 @@
 #define KV8_COLS 16u       // query columns of a wave (a row's heads of one kv head, row after row)
 #define KV8_ROW_COLS 32u   // and of a workgroup of many columns
 #define KV8_MAX_SPLIT 256u // parts of one tile's token range
-#define KV8_PART 4u        // floats of a part's row behind its D sums: maximum, sum, and two unused
+#define KV8_PART 4u        // floats of a part's row behind its D sums: maximum, sum, unit, and one unused
+#define KV8_ATTN_HEAD 768u // bytes of LDS before the few-column kernel's digits: maxima, sums and units
 #define KV8_Q_HEADS 4u     // query heads of one append workgroup
 
 // The cache (gh_kv8_cache); page_tokens = 1 << page_shift.

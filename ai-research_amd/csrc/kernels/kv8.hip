@@ -398,11 +398,16 @@ __device__ __forceinline__ void append(const Kv8AppendArgs& a) {
 // S^T leaves a lane the scores of tokens 4 g .. 4 g + 3 (g = lane / 16) of both
 // 16-token blocks of a step for its column, which is the B operand of the
 // second product: P needs no exchange between lanes.
-// P's halves hold p 2^(14 + e - E) with E the largest scale exponent so far, so
-// that they neither overflow nor lose small probabilities.
+// P's halves hold the column's weights p 2^e (e its block's scale exponent) in units
+// that follow the largest of them so far, which is over 2^14 units (2^10 in the kernel of
+// many columns) and at most 2^15: half a step of the lower half, 2^-25 units, may be lost of
+// each.  Blocks that a column does not see, or sees with little weight, do not move its
+// unit, whatever their scales are.
 // ---------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kNoExp = -100000;
+constexpr float kNoMax = -3.402823466e38f;  // maximum and unit of a column that has seen nothing
+constexpr float kNoUnit = -100000.f;
+constexpr int kTop = 15;  // the largest weight is at most 2^kTop units
 constexpr int kLazy = 4;  // of the kernel of many columns
 
 __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
@@ -506,12 +511,14 @@ __device__ __forceinline__ void load_codes(const Kv8AttnArgs& a, const Tile& t, 
   }
 }
 
-// A column's running softmax, and its sums in units of 2^(E - 14).
+// A column's running softmax: m is what is subtracted from its scores, l their sum, and o
+// the sums of weights 2^(s - m + e) times codes, in units of 2^(E - kTop + LAZY); unit is
+// one over that (0: no weight yet; infinite where f32 does not hold it).  m and E are whole
+// numbers, so that their changes turn the sums by powers of two.
 template <int NL>
 struct Run {
   f32x4 o[NL][4];
-  float m, l;
-  int E;
+  float m, l, E, unit;
 };
 
 template <int NL>
@@ -520,9 +527,10 @@ __device__ __forceinline__ void clear(Run<NL>* r) {
   for (int l = 0; l < NL; l++)
 #pragma unroll
     for (int j = 0; j < 4; j++) r->o[l][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  r->m = -INFINITY;
+  r->m = kNoMax;
   r->l = 0.f;
-  r->E = kNoExp;
+  r->E = kNoUnit;
+  r->unit = 0.f;
 }
 
 // The four digit sums of a score.  Two at a time are exact as integers (at most
@@ -557,60 +565,76 @@ __device__ __forceinline__ bool scale_number(float v) {
 
 // The softmax of a step's scores sc, in units of log2 (-inf: not seen): the halves
 // of P for the second product, and the running values.  vs: the blocks' scales of V.
-// What is subtracted from the scores follows their maximum when that is over it by
-// more than LAZY, so P is at most 2^LAZY (and its halves are in units that much
-// larger): with 16 columns one or another has a new maximum in most steps of a
-// prompt, and each costs a product for every sum.
+// What is subtracted from the scores follows their maximum, and the unit the largest
+// weight, when those are over them by more than LAZY, so P is at most 2^LAZY (and its
+// halves are in units that much larger): with 16 columns one or another has a new maximum
+// in most steps of a prompt, and each costs a product for every sum.  (Prompts of 2000
+// tokens: LAZY 4 108 us, 2 109, 1 and 0 112; what is lost is 2^-35 of the largest weight
+// then, far below f32's 2^-24.)
 template <int NL, int LAZY>
 __device__ __forceinline__ void soft_step(const float (&sc)[2][4], const float (&vs)[2], const bool (&has)[2], Run<NL>* r,
                                           f16x8* phi, f16x8* plo) {
-  float mx = sc[0][0], vmul[2];
-  int E = r->E;
+  float e[2], v[2], mx[2];  // the blocks' scales that count (0: none) and their exponents
 #pragma unroll
   for (int b = 0; b < 2; b++) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[b][i]);
-    // the exponent of a scale that counts (a power of two; 0 has none)
     const uint32_t bits = __builtin_amdgcn_readfirstlane(__float_as_uint(vs[b]));
-    if (has[b] && bits - 1u < 0x7f800000u - 1u) E = max(E, (int)(bits >> 23) - 127);
+    const bool some = has[b] && bits - 1u < 0x7f800000u - 1u;
+    e[b] = some ? (float)((int)(bits >> 23) - 127) : -INFINITY;
+    v[b] = some ? __uint_as_float(bits) : 0.f;
+    mx[b] = fmaxf(fmaxf(sc[b][0], sc[b][1]), fmaxf(sc[b][2], sc[b][3]));
   }
-  mx = column_max(mx);
-  mx = mx > r->m + LAZY ? mx : r->m;
-  const float base = mx == -INFINITY ? 0.f : mx;
-  const float alpha = __builtin_amdgcn_exp2f(r->m - base);
-  const float turn = r->E == E ? alpha : alpha * ldexpf(1.f, max(r->E - E, -200));
-  r->m = mx;
-  r->E = E;
+  const float top = fmaxf(mx[0], mx[1]), most = fmaxf((mx[0] - r->m) + e[0], (mx[1] - r->m) + e[1]);
+  if (__any(top > r->m + LAZY || most > r->E + LAZY)) {
+    const float t = column_max(top), m = t > r->m + LAZY ? ceilf(t) : r->m;
+    const float w = column_max(fmaxf((mx[0] - m) + e[0], (mx[1] - m) + e[1]));
+    const float by = r->m - m, moved = fmaxf(r->E + by, kNoUnit), E = w > moved + LAZY ? ceilf(w) : moved;
+    const float turn = __builtin_amdgcn_exp2f(by + (r->E - E));
+    r->l *= __builtin_amdgcn_exp2f(by);
+    r->m = m;
+    r->E = E;
+    r->unit = E == kNoUnit ? 0.f : ldexpf(1.f, kTop - LAZY - (int)E);
+    if (__any(turn != 1.f)) {
 #pragma unroll
-  for (int b = 0; b < 2; b++) vmul[b] = has[b] && scale_number(vs[b]) ? ldexpf(vs[b], E == kNoExp ? 0 : 14 - LAZY - E) : 0.f;
-  if (__any(turn != 1.f)) {
+      for (int l = 0; l < NL; l++)
 #pragma unroll
-    for (int l = 0; l < NL; l++)
+        for (int j = 0; j < 4; j++) r->o[l][j] *= turn;
+    }
+  }
+  float w[2][4], sum = 0.f;
+  bool far = false;
 #pragma unroll
-      for (int j = 0; j < 4; j++) r->o[l][j] *= turn;
+  for (int b = 0; b < 2; b++) {
+    const float mul = v[b] * r->unit;
+    far |= !(mul <= 0x1p90f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float p = __builtin_amdgcn_exp2f(sc[b][i] - r->m);
+      sum += p;
+      w[b][i] = p * mul;
+    }
+  }
+  // (a scale so far over the unit that only a p below f32's range makes a weight of it)
+  if (__any(far)) {
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        w[b][i] = __builtin_amdgcn_exp2f((sc[b][i] - r->m) + (e[b] - r->E + (float)(kTop - LAZY)));
   }
   union {
     f16x2 h[4];
     f16x8 v;
   } hi, lo;
-  float sum = 0.f;
 #pragma unroll
-  for (int b = 0; b < 2; b++) {
-    float w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float p = __builtin_amdgcn_exp2f(sc[b][i] - base);
-      sum += p;
-      w[i] = p * vmul[b];
-    }
+  for (int b = 0; b < 2; b++)
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      const f16x2 h = half2(w[2 * i], w[2 * i + 1]);
+      const float x = w[b][2 * i], y = w[b][2 * i + 1];
+      const f16x2 h = half2(x, y);
       hi.h[2 * b + i] = h;
-      lo.h[2 * b + i] = half2(w[2 * i] - (float)h[0], w[2 * i + 1] - (float)h[1]);
+      lo.h[2 * b + i] = half2(x - (float)h[0], y - (float)h[1]);
     }
-  }
-  r->l = r->l * alpha + sum;
+  r->l += sum;
   *phi = hi.v;
   *plo = lo.v;
 }
@@ -816,13 +840,17 @@ __device__ __forceinline__ float stage_q(const f32x4 (&x)[(NL + 3) / 4][4], floa
   return bad ? __builtin_nanf("") : ldexpf(1.f, e - 30);
 }
 
-// A lane's sums of its column (dims d0 + 16 g + 4 i .. for each i), times by.
-__device__ __forceinline__ void write_dims(const f32x4 (&o)[4], float* to, uint32_t d0, uint32_t D, float by) {
+// A lane's sums of its column (dims d0 + 16 g + 4 i .. for each i), times by 2^n (in that
+// order: a result below f32's normal range is rounded once).
+__device__ __forceinline__ void write_dims(const f32x4 (&o)[4], float* to, uint32_t d0, uint32_t D, float by, int n) {
   const uint32_t g = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const uint32_t d = d0 + 16 * g + 4 * i;
-    if (d < D) *reinterpret_cast<f32x4*>(to + d) = f32x4{o[0][i], o[1][i], o[2][i], o[3][i]} * by;
+    f32x4 x;
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = ldexpf(o[j][i] * by, n);
+    if (d < D) *reinterpret_cast<f32x4*>(to + d) = x;
   }
 }
 
@@ -845,10 +873,10 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   if (split > 0 && s0 >= end) return;
   const uint32_t s1 = min(s0 + per, end);
 
-  float* lm = reinterpret_cast<float*>(lds);         // [4][16]
-  float* ll = lm + 64;                               // [4][16]
-  i32x4* qd = reinterpret_cast<i32x4*>(lds + 512);   // [4][NL][64]
-  f32x4* lo = reinterpret_cast<f32x4*>(lds + 512);   // [4 waves][NL][4][64 lanes], after the steps
+  float* lm = reinterpret_cast<float*>(lds);                   // [4][16]
+  float *ll = lm + 64, *le = ll + 64;                          // [4][16]
+  i32x4* qd = reinterpret_cast<i32x4*>(lds + KV8_ATTN_HEAD);   // [4][NL][64]
+  f32x4* lo = reinterpret_cast<f32x4*>(lds + KV8_ATTN_HEAD);   // [4 waves][NL][4][64 lanes], after the steps
   uint32_t pages = step_pages(a, t, s0 + wave, 4);
   const uint32_t col = t.col0 + min(n, t.ncol - 1);  // columns past the last repeat it
   f32x4 row[(NL + 3) / 4][4];
@@ -883,38 +911,43 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
   r.l += __shfl_xor(r.l, 16, 64);
   r.l += __shfl_xor(r.l, 32, 64);
 
-  // Join the waves: m and l of all, then each wave the sums of a quarter of the dims.
+  // Join the waves: m, l and E of all, then each wave the sums of a quarter of the dims.
   if (lane < 16) {
     lm[wave * 16 + n] = r.m;
     ll[wave * 16 + n] = r.l;
+    le[wave * 16 + n] = r.E;
   }
   __syncthreads();
-  float M = -INFINITY, L = 0.f;
+  float M = kNoMax, L = 0.f, E = kNoUnit;
 #pragma unroll
   for (int w = 0; w < 4; w++) M = fmaxf(M, lm[w * 16 + n]);
-  const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
-  for (int w = 0; w < 4; w++) L += ll[w * 16 + n] * __builtin_amdgcn_exp2f(lm[w * 16 + n] - base);
-  // (two factors: the unit of the smallest scales is below f32's normal range)
-  const float f = __builtin_amdgcn_exp2f(r.m - base), unit = r.E == kNoExp ? 0.f : ldexpf(1.f, r.E - 14);
+  for (int w = 0; w < 4; w++) {
+    L += ll[w * 16 + n] * __builtin_amdgcn_exp2f(lm[w * 16 + n] - M);
+    E = fmaxf(E, le[w * 16 + n] + (lm[w * 16 + n] - M));
+  }
+  const float f = __builtin_amdgcn_exp2f((r.m - M) + (r.E - E));
 #pragma unroll
   for (int l = 0; l < NL; l++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) lo[((wave * NL + l) * 4 + j) * 64 + lane] = r.o[l][j] * f * unit;
+    for (int j = 0; j < 4; j++) lo[((wave * NL + l) * 4 + j) * 64 + lane] = r.o[l][j] * f;
   __syncthreads();
   if (n >= t.ncol) return;
   const bool only = per >= t.steps;  // the only split that runs
   float* to;
   float by = 1.f;
+  int unit = 0;
   if (only) {
     to = a.out + row_at(a, t, col);
-    by = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;  // nothing visible: 0
+    by = L == 0.f ? 0.f : 1.f / L;  // nothing visible: 0
+    unit = (int)E - kTop;
   } else {
     const uint64_t place = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / a.nsplit) + tile;
     to = a.part + ((place * a.nsplit + split) * KV8_COLS + n) * (D + KV8_PART);
     if (wave == 0 && g == 0) {
       to[D] = M;
       to[D + 1] = L;
+      to[D + 2] = E;
     }
   }
 #pragma unroll
@@ -928,7 +961,7 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
 #pragma unroll
       for (int w = 1; w < 4; w++) x[j] += lo[((w * NL + l) * 4 + j) * 64 + lane];
     }
-    write_dims(x, to, 64 * l, D, by);
+    write_dims(x, to, 64 * l, D, by, unit);
   }
 }
 
@@ -1077,35 +1110,36 @@ __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
   r.l += __shfl_xor(r.l, 16, 64);
   r.l += __shfl_xor(r.l, 32, 64);
   // the odd steps' sums come to the wave of the even ones
-  const float unit = r.E == kNoExp ? 0.f : ldexpf(1.f, r.E - (14 - kLazy));
-  float* lm = reinterpret_cast<float*>(lds) + part * (16 * NL * 64 + 128);
-  float* lo = lm + 128;
+  float* lm = reinterpret_cast<float*>(lds) + part * (16 * NL * 64 + 192);
+  float* lo = lm + 192;
   if (par == 1) {
     lm[lane] = r.m;
     lm[64 + lane] = r.l;
+    lm[128 + lane] = r.E;
 #pragma unroll
     for (int l = 0; l < NL; l++)
 #pragma unroll
       for (int j = 0; j < 4; j++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) lo[(l * 16 + j * 4 + i) * 64 + lane] = r.o[l][j][i] * unit;
+        for (int i = 0; i < 4; i++) lo[(l * 16 + j * 4 + i) * 64 + lane] = r.o[l][j][i];
   }
   __syncthreads();
   if (par == 1) return;
-  const float m1 = lm[lane], M = fmaxf(r.m, m1), base = M == -INFINITY ? 0.f : M;
-  const float f0 = __builtin_amdgcn_exp2f(r.m - base), f1 = __builtin_amdgcn_exp2f(m1 - base);
-  const float L = r.l * f0 + lm[64 + lane] * f1;
+  const float m1 = lm[lane], M = fmaxf(r.m, m1), d0 = r.m - M, d1 = m1 - M;
+  const float E = fmaxf(fmaxf(r.E + d0, lm[128 + lane] + d1), kNoUnit);
+  const float f0 = __builtin_amdgcn_exp2f(d0 + (r.E - E)), f1 = __builtin_amdgcn_exp2f(d1 + (lm[128 + lane] - E));
+  const float L = r.l * __builtin_amdgcn_exp2f(d0) + lm[64 + lane] * __builtin_amdgcn_exp2f(d1);
 #pragma unroll
   for (int l = 0; l < NL; l++)
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) r.o[l][j][i] = fmaf(lo[(l * 16 + j * 4 + i) * 64 + lane], f1, r.o[l][j][i] * f0 * unit);
+      for (int i = 0; i < 4; i++) r.o[l][j][i] = fmaf(lo[(l * 16 + j * 4 + i) * 64 + lane], f1, r.o[l][j][i] * f0);
   if (c0 + n > last) return;
-  const float by = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;  // nothing visible: 0
+  const float by = L == 0.f ? 0.f : 1.f / L;  // nothing visible: 0
   float* to = a.out + row_at(a, t, col);
 #pragma unroll
-  for (int l = 0; l < NL; l++) write_dims(r.o[l], to, 64 * l, D, by);
+  for (int l = 0; l < NL; l++) write_dims(r.o[l], to, 64 * l, D, by, (int)E - kTop + kLazy);
 }
 
 }  // namespace
@@ -1138,29 +1172,37 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, 
   const uint64_t unit = ((uint64_t)blockIdx.z * a.c.nkv + t.head) * (gridDim.x / cols) + tile;
   const uint64_t row = KV8_COLS * (uint64_t)(D + KV8_PART);
   const float* p = a.part + unit * a.nsplit * row + n * (uint64_t)(D + KV8_PART);
-  __shared__ float f[KV8_MAX_SPLIT], red[8];
+  __shared__ float f[KV8_MAX_SPLIT], red[12];
   constexpr uint32_t N = 8;  // sums on their way at a time, the first of them before the factors
   float x[N];
 #pragma unroll
   for (uint32_t i = 0; i < N; i++) x[i] = i < live && tid < D ? p[i * row + tid] : 0.f;
-  float m = -INFINITY, l = 0.f;
+  float m = kNoMax, l = 0.f, e = kNoUnit;
   if (tid < live) {
     m = p[tid * row + D];
     l = p[tid * row + D + 1];
+    e = p[tid * row + D + 2];
   }
-  float M = m;
+  // the largest maximum, and the largest unit (one that rounding shifts is as good)
+  float M = m, E = m + e;
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
-  if ((tid & 63) == 0) red[tid >> 6] = M;
+  for (int off = 32; off > 0; off >>= 1) {
+    M = fmaxf(M, __shfl_xor(M, off, 64));
+    E = fmaxf(E, __shfl_xor(E, off, 64));
+  }
+  if ((tid & 63) == 0) {
+    red[tid >> 6] = M;
+    red[8 + (tid >> 6)] = E;
+  }
   __syncthreads();
   M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float base = M == -INFINITY ? 0.f : M, w = __builtin_amdgcn_exp2f(m - base);
-  f[tid] = w;
-  const float L0 = wave_sum(l * w);
+  E = fmaxf(fmaxf(fmaxf(red[8], red[9]), fmaxf(red[10], red[11])) - M, kNoUnit);
+  f[tid] = __builtin_amdgcn_exp2f((m - M) + (e - E));
+  const float L0 = wave_sum(l * __builtin_amdgcn_exp2f(m - M));
   if ((tid & 63) == 0) red[4 + (tid >> 6)] = L0;
   __syncthreads();
   const float L = (red[4] + red[5]) + (red[6] + red[7]);
-  const float by = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;
+  const float by = L == 0.f ? 0.f : 1.f / L;
   float* out = a.out + row_at(a, t, t.col0 + n);
   for (uint32_t d = tid; d < D; d += 256) {
     float o = 0.f;
@@ -1172,7 +1214,7 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, 
 #pragma unroll
       for (uint32_t i = 0; i < N; i++) o = fmaf(x[i], s + i < live ? f[s + i] : 0.f, o);
     }
-    out[d] = o * by;
+    out[d] = ldexpf(o * by, (int)E - kTop);
   }
 }
 

@@ -300,7 +300,8 @@ gh_status gh_kv8_attn(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8_b
                              (a.c.D == 64 * nl ? "" : "r") + (p.stream ? "s_k" : "_k");
     void* args[] = {&a};
     if (p.rows) return launch(ctx, name.c_str(), dim3(p.tiles * a.c.nkv, 1, a.b.num_seqs), dim3(256), 14336 * nl, args);
-    st = launch(ctx, name.c_str(), dim3(p.tiles * p.nsplit, a.c.nkv, a.b.num_seqs), dim3(256), 512 + 16384 * nl, args);
+    st = launch(ctx, name.c_str(), dim3(p.tiles * p.nsplit, a.c.nkv, a.b.num_seqs), dim3(256),
+                KV8_ATTN_HEAD + 16384 * nl, args);
     if (st != GH_OK || p.nsplit == 1) return st;
     uint32_t cols = (uint32_t)std::min<uint64_t>(KV8_COLS, (uint64_t)a.b.max_rows * (num_q / a.c.nkv));
     void* margs[] = {&a, &cols};
