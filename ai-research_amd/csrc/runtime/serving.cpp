@@ -2,6 +2,7 @@
 // (append, read-back, attention), probabilities from logits, and the verification
 // of drafted tokens.  Argument checks, launch shapes, and the launch on the
 // context stream.  Nothing here allocates: a caller gives the workspace.
+#include <float.h>
 #include <math.h>
 
 #include <new>
@@ -330,7 +331,10 @@ gh_status gh_logit_probs(gh_context* ctx, const float* logits, float* probs, uin
     gh_status st = check_work(who, work, work_bytes, gh_logit_probs_workspace(ctx, rows, vocab));
     if (st != GH_OK) return st;
     const uint32_t each = sample_each(ctx, rows, vocab);
-    const double mul = 1.4426950408889634 / (double)temperature * (softcap > 0.f ? (double)softcap : 1.0);
+    double mul = 1.4426950408889634 / (double)temperature * (softcap > 0.f ? (double)softcap : 1.0);
+    // (soft-capped logits lie within 2 of each other in units of the cap: a factor below f32's
+    // normal range makes them all even, as that range's least does; 0 would make masked ones NaN)
+    if (softcap > 0.f) mul = std::max(mul, (double)FLT_MIN);
     ProbsArgs a{logits, probs, static_cast<float*>(work), stride, vocab, chunks_of(vocab, each),
                 softcap > 0.f ? 1.f / softcap : 0.f, (float)mul};
     if (!(a.mul < INFINITY)) return invalid(who, "softcap / temperature is too large");
