@@ -135,7 +135,9 @@ gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, co
   if (tiles * c.nkv >= 1ull << 24) return unsupported(who, "2^29 or more query columns");
   p->tiles = (uint32_t)tiles;
   if (p->rows) return GH_OK;
-  uint64_t tokens = (uint64_t)r.max_pages << c.page_shift;
+  // (tokens are numbered in 32 bits: a table of more pages has no use for them, and the parts'
+  // steps are counted in as many)
+  uint64_t tokens = std::min<uint64_t>((uint64_t)r.max_pages << c.page_shift, (1ull << 32) + r.max_rows);
   if (max_kv) tokens = std::min<uint64_t>(tokens, max_kv);
   if (window) tokens = std::min<uint64_t>(tokens, (uint64_t)window + (KV8_COLS + G - 1) / G);
   const uint64_t steps = tokens / KV8_STEP + 1;
