@@ -37,10 +37,12 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 
 // The first launch of a kernel asks the code objects for it in turn; the answer
 // "not found" of one stays behind as HIP's last error, which a host's other HIP
-// code in this thread would take for its own.
+// code in this thread would take for its own.  An error that was pending before is the
+// host's, and stays.
 gh_status launch(gh_context* ctx, const char* name, dim3 grid, dim3 block, unsigned lds, void** args) {
+  const bool clean = hipPeekAtLastError() == hipSuccess;
   const hipFunction_t f = ctx->fn(name);
-  if (hipPeekAtLastError() == hipErrorNotFound) (void)hipGetLastError();
+  if (clean && hipPeekAtLastError() == hipErrorNotFound) (void)hipGetLastError();
   if (!f) return fail(GH_ERR_CODE_OBJECT, std::string("kernel not found in the code objects: ") + name);
   return ctx->launch(name, grid, block, lds, args);
 }

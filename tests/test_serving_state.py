@@ -34,6 +34,11 @@ def state(tmp_path_factory):
     return ask
 
 
+@pytest.mark.parametrize("before,after", [("none", "none"), ("not_found", "some"), ("invalid", "some")])
+def test_errors_of_the_host_stay_pending_and_lookups_leave_none(state, before, after):
+    assert state("error", before) == ["0", after]
+
+
 @pytest.mark.parametrize("pages", [1, 40, 5000, 1 << 20, (1 << 24) + 1, 1 << 28, 1 << 31, 0xffffffff])
 @pytest.mark.parametrize("tokens", [0, 1, 100000, 0xffffffff])
 def test_parts_count_their_steps_in_32_bits(state, pages, tokens):
