@@ -209,6 +209,9 @@ gh_status gh_kv8_append(gh_context* ctx, const gh_kv8_cache* cache, const gh_kv8
     if (num_q && (!Q_in || !Q_norm || !Q_out)) return invalid(who, "Q_in, Q_norm or Q_out is null");
     if (kv_stride < (uint64_t)a.c.nkv * a.c.D || (num_q && q_stride < (uint64_t)num_q * a.c.D))
       return invalid(who, "a row stride is shorter than its heads");
+    if (num_q && Q_out == Q_in && q_stride != (uint64_t)num_q * a.c.D && a.b.num_rows > 1)
+      return invalid(who, "Q_out is Q_in with rows that are not num_q * head_dim apart");
+    if (num_q && (Q_out == K_in || (Q_out == V_in && !k_eq_v))) return invalid(who, "Q_out is K_in or V_in");
     for (const void* p : {(const void*)Q_in, (const void*)K_in, (const void*)V_in, (const void*)Q_norm,
                           (const void*)K_norm, (const void*)Q_out})
       if (!aligned(p, 4)) return invalid(who, "rows and norms must be 4-byte aligned");

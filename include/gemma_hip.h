@@ -336,7 +336,8 @@ typedef struct gh_kv8_batch {
  * unit-RMS of each value head (the raw key head when k_eq_v) into the cache at
  * the row's token.  Q_in has rows q_stride floats apart, K_in and V_in kv_stride
  * (they may lie in one packed [q|k|v] row); Q_out may be Q_in when q_stride is
- * num_q * head_dim.  num_q 0 appends only.  Angles, keys and values are computed
+ * num_q * head_dim (or num_rows 1), and is refused otherwise, as K_in and as a
+ * V_in that is read.  num_q 0 appends only.  Angles, keys and values are computed
  * in 64 bits up to the code (half to even).
  *
  * A block's scale is the least power of two whose 127-fold reaches the largest
