@@ -396,9 +396,16 @@ def _i32(*shape):
     return torch.empty(shape, dtype=torch.int32, device="cuda")
 
 
+_HELD = ("k", "v", "k_scale", "v_scale", "seq_start", "past_len", "pages", "read_start", "read_past")
+
+
 def _handles(s):
-    """What a host makes once for a state: descriptors, result buffers and workspace."""
+    """What a host makes once for a state's tensors: descriptors, result buffers and workspace.
+
+    The context has a stream of its own: what torch still has to write of the inputs is waited for here, once.
+    """
     gh, ctx = _binding()
+    torch.cuda.current_stream().synchronize()
     case, kind = s["case"], s["case"]["kind"]
     p = lambda t: t.data_ptr()  # noqa: E731
     h = dict(ctx=ctx)
@@ -409,6 +416,7 @@ def _handles(s):
         h["out"] = dict(tokens=_i32(case["seqs"], case["draft"] + 1), accepted=_i32(case["seqs"]))
         h["bytes"] = ctx.spec_verify_workspace(case["seqs"], case["vocab"])
     else:
+        h.update({n: s.get(n) for n in _HELD})  # (whose addresses the descriptors hold)
         h["cache"] = gh.Kv8Cache(p(s["k"]), p(s["v"]), p(s["k_scale"]), p(s["v_scale"]), s["k"].shape[0], case["page"],
                                  case["kv_heads"], case["head_dim"])
         h["batch"] = gh.Kv8Batch(p(s["seq_start"]), p(s["past_len"]), p(s["pages"]), case["seqs"], s["pages"].shape[1],
@@ -428,9 +436,14 @@ def _handles(s):
 
 
 def _run_own(s):
-    if "handles" not in s:
-        s["handles"] = _handles(s)
-    h, case, kind = s["handles"], s["case"], s["case"]["kind"]
+    """The calls, on the context's stream: results (the state's buffers, until its next run) and what else
+    the call wrote are there for torch once the device has been waited for."""
+    h, case, kind = s.get("handles"), s["case"], s["case"]["kind"]
+    if h is None or kind in ("append", "attn") and not (
+            s["k"] is h["k"] and s["v"] is h["v"] and s["k_scale"] is h["k_scale"] and s["v_scale"] is h["v_scale"] and
+            s["seq_start"] is h["seq_start"] and s["past_len"] is h["past_len"] and s["pages"] is h["pages"] and
+            (kind == "attn" or s["read_start"] is h["read_start"] and s["read_past"] is h["read_past"])):
+        h = s["handles"] = _handles(s)
     p = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
     ctx, out, work, size = h["ctx"], h["out"], p(h.get("work")), h.get("bytes", 0)
     if kind == "probs":
