@@ -547,10 +547,6 @@ __device__ __forceinline__ float column_max(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-__device__ __forceinline__ float uniform(float x) {
-  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
-}
-
 // Two numbers as f16, to nearest.
 __device__ __forceinline__ f16x2 half2(float a, float b) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
