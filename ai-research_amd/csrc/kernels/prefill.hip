@@ -522,14 +522,12 @@ struct WQ4 {
   // 1/16 and -72, leaves n - 8.  So only the upper half of the word is shifted.
   __device__ static uint32_t pair(const uint32_t* w, int p, const Unpack& c) {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    uint32_t pr;
-    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(pr) : "v"(p < 2 ? w[0] : w[0] >> 8), "v"(p % 2 ? c.hi : c.lo), "s"(c.magic));
-    const h2 v = __builtin_bit_cast(h2, pr);
+    const h2 v = __builtin_bit_cast(h2, ((p < 2 ? w[0] : w[0] >> 8) & (p % 2 ? c.hi : c.lo)) | c.magic);
     h2 o;
     if (p % 2 == 0)
       o = v + h2{(_Float16)-1032.0f, (_Float16)-1032.0f};
     else
-      asm("v_pk_fma_f16 %0, %1, %2, %3" : "=v"(o) : "v"(v), "v"(c.sixteenth), "s"(c.bias));
+      o = __builtin_elementwise_fma(v, __builtin_bit_cast(h2, c.sixteenth), __builtin_bit_cast(h2, c.bias));
     return __builtin_bit_cast(uint32_t, o);
   }
 };
