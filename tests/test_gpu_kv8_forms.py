@@ -96,3 +96,37 @@ def test_attention_of_prompts_by_bounds(gpu, nq, H, D, page, rows, past, window,
             assert np.all(np.abs(got[at + i:at + i + 1] - want) <= bound), (b, i)
         assert np.all(got[at + live:at + n] == 5.0), b
         at += n
+
+
+# ---- a cache of more than 4 GiB --------------------------------------------------------------
+def test_pages_past_32_bits_of_bytes(gpu):
+    """Codes of 4.3 GiB each of keys and values, of which only the last pages and the first are named, against the
+    same calls on a small cache: the same bits."""
+    nq, H, D, page = 8, 4, 512, 64
+    pages = (1 << 32) // (page * H * D) + 2000
+    rng = np.random.default_rng(77)
+    rows, past = [70, 3], [0, 0]
+    qkv, qn, kn = packed_rows(rng, sum(rows), nq, H, D)
+    w, sides = (nq + 2 * H) * D, []
+    for n, names in ((4, [3, 0, 2, 1]), (pages, [pages - 1, 0, pages - 2, pages - 1000])):
+        tables = np.array([[names[0], names[1]], [names[2], names[3]]], np.uint32)
+        c = gh.Kv8Cache(None, None, None, None, n, page, H, D)
+        codes, scales = gh.lib().gh_kv8_code_bytes(c), gh.lib().gh_kv8_scale_bytes(c)
+        assert codes == n * page * H * D and (n == 4 or codes > 1 << 32)
+        held = [gpu.alloc(b) for b in (codes, codes, scales, scales)]
+        c.k, c.v, c.k_scale, c.v_scale = (h.ptr for h in held)
+        start, P, T = (gpu.upload(np.asarray(a, np.uint32)) for a in (np.concatenate([[0], np.cumsum(rows)]), past, tables))
+        b = gh.Kv8Batch(start.ptr, P.ptr, T.ptr, 2, 2, sum(rows), max(rows))
+        X, QN, KN, Q = gpu.upload(qkv), gpu.upload(qn), gpu.upload(kn), gpu.alloc(sum(rows) * nq * D * 4)
+        gpu.kv8_append(c, b, X.ptr, X.ptr + 4 * nq * D, X.ptr + 4 * (nq + H) * D, w, w, QN, KN, Q, nq, D, False, 10000.0, EPS)
+        K, V, O = (gpu.alloc(sum(rows) * h * D * 4) for h in (H, H, nq))
+        gpu.kv8_read(c, b, K, V)
+        size = gpu.kv8_attn_workspace(c, b, nq, 0, 70)
+        W = gpu.alloc(max(size, 16))
+        gpu.kv8_attn(c, b, Q, O, nq, 0.0442, 0, 70, W, size)
+        sides.append([x.read(np.uint32) for x in (Q, K, V, O)])
+        for h in held:
+            h.free()
+    for one, two in zip(*sides):
+        assert np.array_equal(one, two)
+    assert np.isfinite(sides[0][3].view(np.float32)).all()
