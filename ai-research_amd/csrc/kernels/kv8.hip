@@ -119,8 +119,9 @@ __device__ __forceinline__ void pair_dims(uint32_t i, uint32_t D, uint32_t rot, 
 // far out: two sines and cosines per pair and a run of rows, the rows between by
 // rotating on.  What a workgroup waits for is on its way before it computes the
 // angles: the whole of its rows, and the codes already there.  (2000 rows of 16 query
-// and 8 key heads of 256: 35 us, 3 TB/s; the vector units are busy for 56% of it, and
-// the waves, four a SIMD, wait for as long.  One row: 5 us.)
+// and 8 key heads of 256: 34 us, 3.1 TB/s; the vector units are busy for 58% of it, and
+// the waves, four a SIMD, wait for 54%.  Every head's workgroup works out the angles of its
+// block anew.  One row: 5 us.)
 // ---------------------------------------------------------------------------
 struct Angle {
   double c, s;
@@ -854,7 +855,7 @@ __device__ __forceinline__ void write_dims(const f32x4 (&o)[4], float* to, uint3
 // tokens' bytes bound it, so a wave has the next step's keys on the way while it
 // weighs this step's values, and the next values while it scores; the query
 // digits are in LDS to leave the registers to them.  (Heads of 256 over 8 key heads: 32
-// rows over 20 - 4000 tokens 55 us, 4.8 TB/s of codes; one row over 120000 78 us, 6.3.)
+// rows over 20 - 4000 tokens 55 us, 4.8 TB/s of codes; one row over 120000 80 us, 6.2.)
 // grid (tiles * splits, kv heads, sequences)
 template <int NL, bool FULL, bool STREAM>
 __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
@@ -970,8 +971,9 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
 // over the CUs.  The codes of a step come through LDS once for its two waves, the values'
 // already as f16, whose conversion is as much vector work as the softmax; the next
 // step's are on their way to registers meanwhile.  (A prompt of 2000 tokens, 16 heads of
-// 256 over 8 key heads: 99 us, 66 GFLOP made, the matrix cores busy for 32% of it;
-// with 64 columns a workgroup 96 us, but prompts of 350 - 650 tokens 13 - 20% slower.)
+// 256 over 8 key heads: 95 us, 66 GFLOP made, the matrix cores busy for 32% of it, the
+// vector units for 50%.  64 columns a workgroup took 3% less, but 13 - 20% more for prompts of
+// 350 - 650 tokens.)
 // grid (tiles * kv heads, 1, sequences), the tiles that see most first; the heads in
 // turn, so that with eight of them a head's workgroups share an XCD's L2.
 template <int NL, bool FULL>

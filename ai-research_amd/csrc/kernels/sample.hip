@@ -44,7 +44,7 @@ __device__ __forceinline__ void load_chunk(const float* row, uint32_t c, uint32_
 // Probabilities: y = cap tanh(x / cap) (x without a cap; -inf stays), p =
 // 2^((y - max) log2(e) / temperature) / sum.  The first launch leaves each chunk's
 // maximum and sum, the second joins a row's and writes; it finds the logits in
-// the last-level cache.  (40 rows of 262144: 20 us a call among others, 23 when the
+// the last-level cache.  (40 rows of 262144: 19 us a call among others, 23 when the
 // second's loads and stores stay in the caches; 4 bytes read and 4 written an element
 // at the rate of a copy are 17.7.)
 // ---------------------------------------------------------------------------
@@ -177,7 +177,7 @@ __device__ __forceinline__ void probs_write(const ProbsArgs& a) {
 // where it stops, the token is drawn from what the target has over the draft,
 // max(p - q, 0), or from the target itself after the last draft.  A token is
 // decided next to a border, so weights and sums are in 64 bits.  (32 sequences of 262144:
-// 12.6 us for the chunks' sums, 5.3 TB/s, and 5.2 for the token, a chain of loads.)
+// 12.9 us for the chunks' sums, 5.2 TB/s, and 4.9 for the token, a chain of loads.)
 // ---------------------------------------------------------------------------
 struct Stop {
   uint32_t kept, drafts;

@@ -103,25 +103,27 @@ struct AttnPlan {
 // workgroups: it is taken where several tiles of 16 columns a sequence alone give every CU
 // two of them.
 // (us with it and with the other one, 8 key heads of 256 under 16 query heads: prompts
-// of 2000 tokens 98 / 120, 700: 31 / 32, 8 of 64 rows over 1000: 41 / 47, over 4000: 123
-// / 158; with fewer tiles, a prompt of 500: 24 / 20, 8 of 32 over 2000: 47 / 45; with one
-// tile, 100 single rows over 500 - 3000: 177 / 135.)
+// of 2000 tokens 107 / 121, 700: 32 / 32, 8 of 64 rows over 1000: 45 / 49, over 4000: 133
+// / 169; with fewer tiles, a prompt of 500: 26 / 20, 8 of 32 over 2000: 71 / 44; with one
+// tile, 100 single rows over 500 - 3000: 176 / 135.)
 //
 // The other one splits the tokens where that shortens the whole: its four waves take
 // steps of 32 tokens in turn, 2.3 us for a step each (256 dims; 0.6 more of that for
 // every workgroup that some CU has beyond one), and the splits' sums cost a launch and their
-// way through memory, 4 us and 3 TB/s.  (One token over 544, 8 heads: 5 splits 10.9 us,
-// none 13.7; 8 sequences of 32 rows over 2000, 256 tiles: none 45, 2 58; a prompt of 256
-// tokens, 256 tiles: none 11, 2 22; 32 sequences of 20 - 4000 tokens, 256 tiles: 2 66,
-// none 78; 8 of 5 rows over 1000 - 3000, 64 tiles: 6 24, none 49.)  Parts are of equal
+// way through memory, 4 us and 3 TB/s.  (One token over 544, 8 heads: 5 splits 11.2 us,
+// none 13.6; 8 sequences of 32 rows over 2000, 256 tiles: none 44, 2 61; a prompt of 256
+// tokens, 256 tiles: none 11, 2 23; 32 sequences of 20 - 4000 tokens, 256 tiles: 2 60,
+// none 70; 8 of 5 rows over 1000 - 3000, 64 tiles: 8 24, none 47.  The estimate is for loads
+// through the caches, and can be a tenth off for those by them: the 32 sequences take 57
+// with 3, and of 4000 tokens each 87 with none against 92.)  Parts are of equal
 // length in tokens, so that long sequences of a batch take more of them than short ones.
 // They are at most as many as two workgroups a CU, which even out lengths that differ; one
-// a CU where there is one sequence and tile (one row over 120000 tokens: 85 us with one, 90
-// with two; over 30000: 31 and 33).
+// a CU where there is one sequence and tile (one row over 120000 tokens: 85 us with one, 89
+// with two; over 30000: 31 and 32).
 //
 // Codes that one tile reads once, and that are too many to be in the last-level cache
 // (256 MB) at the next call, pass by the caches: from 96 MB on, going by the bounds.  (One
-// row over 120000, 492 MB: 85 us by them and 94 through them; 16 sequences over 2000,
+// row over 120000, 492 MB: 85 us by them and 98 through them; 16 sequences over 2000,
 // 131 MB: 30 and 34; 8 over 2000, 65 MB, the same three caches in turn: 21 and 20.)
 gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, const Kv8Rows& r, uint32_t num_q,
                     uint32_t window, uint32_t max_kv, AttnPlan* p) {
@@ -163,8 +165,10 @@ gh_status plan_attn(const char* who, const gh_context* ctx, const Kv8View& c, co
 }
 
 // Elements of a thread in the sampling kernels: 16, or 4 while that gives fewer
-// workgroups than CUs (one row of 262144: probabilities 7.5 us
-// with 4 a thread, 9.9 with 16; verification 8.7 and 10.9).
+// workgroups than CUs (one row of 262144, least times of the two launches: probabilities
+// 2.7 + 3.0 us with 4 a thread, 3.1 + 4.0 with 16; verification 3.2 + 2.6 and 3.5 + 4.3;
+// the calls take 7 and 8 us, what a host needs to launch them.  40 rows: 26 us with 4, 20 with
+// 16; verification of 32: 22 and 18).
 uint32_t sample_each(const gh_context* ctx, uint32_t rows, uint32_t vocab) {
   const uint64_t many = (vocab + 256ull * SAMPLE_MANY - 1) / (256 * SAMPLE_MANY);
   return rows * many < (uint64_t)ctx->num_cus ? SAMPLE_FEW : SAMPLE_MANY;
