@@ -1181,23 +1181,24 @@ extern "C" __global__ __launch_bounds__(256) void gh_kv8_merge_k(Kv8AttnArgs a, 
     l = p[tid * row + D + 1];
     e = p[tid * row + D + 2];
   }
-  // the largest maximum, and the largest unit (one that rounding shifts is as good)
-  float M = m, E = m + e;
+  // the largest maximum, then the largest unit by it
+  float M = m;
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    M = fmaxf(M, __shfl_xor(M, off, 64));
-    E = fmaxf(E, __shfl_xor(E, off, 64));
-  }
+  for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+  if ((tid & 63) == 0) red[tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float x2 = (m - M) + e, L0 = wave_sum(l * __builtin_amdgcn_exp2f(m - M));
+  float E = fmaxf(x2, kNoUnit);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) E = fmaxf(E, __shfl_xor(E, off, 64));
   if ((tid & 63) == 0) {
-    red[tid >> 6] = M;
+    red[4 + (tid >> 6)] = L0;
     red[8 + (tid >> 6)] = E;
   }
   __syncthreads();
-  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  E = fmaxf(fmaxf(fmaxf(red[8], red[9]), fmaxf(red[10], red[11])) - M, kNoUnit);
-  f[tid] = __builtin_amdgcn_exp2f((m - M) + (e - E));
-  const float L0 = wave_sum(l * __builtin_amdgcn_exp2f(m - M));
-  if ((tid & 63) == 0) red[4 + (tid >> 6)] = L0;
+  E = fmaxf(fmaxf(red[8], red[9]), fmaxf(red[10], red[11]));
+  f[tid] = __builtin_amdgcn_exp2f(x2 - E);
   __syncthreads();
   const float L = (red[4] + red[5]) + (red[6] + red[7]);
   const float by = L == 0.f ? 0.f : 1.f / L;

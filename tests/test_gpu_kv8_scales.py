@@ -132,6 +132,25 @@ def test_parts_with_units_of_their_own(gpu, drop, small, large):
     check(run_attn(gpu, dev, rows, past, tables, q, scale, 0), want, bound)
 
 
+@pytest.mark.parametrize("size", [1.0, 1e9, 1e30])
+def test_parts_of_scores_past_all_units(gpu, size):
+    # equal scores of any size are an average of the values, also of values near f32's end
+    nq, D, page = 2, 64, 16
+    rng = np.random.default_rng(11)
+    cache = ref.Cache(260, page, 1, D, rng)
+    cache.codes[0][:], cache.scales[0][:], cache.scales[1][:] = 1, 1.0, 2.0 ** 110
+    cache.codes[1][:] = rng.integers(100, 128, cache.codes[1].shape)
+    dev = ref.Device(gpu, cache)
+    tables = np.arange(260, dtype=np.uint32)[None]
+    q = np.full((1, nq, D), size, np.float32)
+    b = dev.batch([1], [4149], tables)
+    assert gpu.kv8_attn_workspace(dev.cache, b, nq, 0, 0) > 0
+    got = run_attn(gpu, dev, [1], [4149], tables, q, 1.0, 0)
+    values = cache.rows(1, tables[0], 0, 4150)[0][:, 0]
+    # (weights are equal up to the exponentials' 4 half steps and the sums' n / 4 + 64, as above)
+    assert np.all(np.abs(got[0] - values.mean(0)) <= 2 * (4 + 8 + 4150 / 4 + 64) * U * values.mean(0))
+
+
 @pytest.mark.parametrize("D", [64, 256])
 def test_a_prompt_with_blocks_far_apart(gpu, D):
     # causal rows over values of every size: each row as precise as its own
