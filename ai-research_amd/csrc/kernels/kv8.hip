@@ -554,8 +554,7 @@ __device__ __forceinline__ f16x2 half2(float a, float b) {
   return __builtin_convertvector((f32x2{a, b}), f16x2);
 }
 
-// The scale that a block's scores take: NaN where its values' scale is no number, so
-// that what sees one of them is NaN.  (Uniform; 0 where there is no page.)
+// Whether a block's scale is a number (uniform).
 __device__ __forceinline__ bool scale_number(float v) {
   return (uint32_t)__builtin_amdgcn_readfirstlane(__float_as_uint(v)) < 0x7f800000u;
 }
@@ -650,16 +649,47 @@ __device__ __forceinline__ void settle(i32x4 (&acc)[2][4]) {
                  "+v"(acc[1][2]), "+v"(acc[1][3]));
 }
 
+// What digit sums are multiplied with, but for their block's scale: a lane's column's unit and
+// the constants, times 2^lift, which the scales are divided by.
+struct Factor {
+  float mul;
+  int lift;
+};
+
+// Of digits in units of 2^e (odd: of a row with a NaN or an infinity).  Queries so small that their
+// factor is below f32's range (x < -125) have scores that count only under scales far above 1, and
+// lend that range to them, as far as the wave's largest queries can do without scales below
+// 2^(lift - 126).
+__device__ __forceinline__ Factor factor_of(int e, bool odd, float scale) {
+  const float c = scale * kLog2e;
+  const int x = e + (int)((__float_as_uint(c) >> 23) & 255u) - 127;
+  Factor f{0.f, 0};
+  if (__any(!odd && x < -125)) {
+    int most = odd ? -1000 : x;
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) most = max(most, __shfl_xor(most, off, 64));
+    f.lift = __builtin_amdgcn_readfirstlane(min(80, max(0, 49 - most)));
+  }
+  f.mul = odd ? __builtin_nanf("") : ldexpf(c, e + f.lift);
+  return f;
+}
+
 // Scores, in units of log2, from their digit sums; -inf: not seen.
 __device__ __forceinline__ void finish_scores(const Kv8AttnArgs& a, i32x4 (&acc)[2][4], const float (&ks)[2],
-                                              const float (&vs)[2], const bool (&has)[2], float qmul, const Tile& t,
+                                              const float (&vs)[2], const bool (&has)[2], Factor f, const Tile& t,
                                               int64_t pos, uint32_t step, float (&sc)[2][4]) {
   const uint32_t g = (threadIdx.x & 63) >> 4;
   settle(acc);
+  float by[2] = {ks[0], ks[1]};
+  if (f.lift != 0) {
+#pragma unroll
+    for (int b = 0; b < 2; b++) by[b] = ldexpf(by[b], -f.lift);
+  }
 #pragma unroll
   for (int b = 0; b < 2; b++) {
-    // (powers of two and the constant: one rounding, of the constant)
-    const float mul = qmul * (scale_number(vs[b]) ? ks[b] : __builtin_nanf(""));
+    // (powers of two and the constant: one rounding, of the constant.  NaN where a scale of the
+    // block is no number, so that what sees one of its tokens is NaN)
+    const float mul = f.mul * (scale_number(vs[b]) ? by[b] : __builtin_nanf(""));
 #pragma unroll
     for (int i = 0; i < 4; i++) sc[b][i] = digit_sum(acc[b][3][i], acc[b][2][i], acc[b][1][i], acc[b][0][i]) * mul;
   }
@@ -677,7 +707,7 @@ __device__ __forceinline__ void finish_scores(const Kv8AttnArgs& a, i32x4 (&acc)
 // Scores of a step's tokens 4 g .. of both blocks for a lane's column.
 template <int NL>
 __device__ __forceinline__ void score_step(const Kv8AttnArgs& a, const Codes<NL>& k, const float (&vs)[2], const i32x4* qd,
-                                           float qmul, const Tile& t, int64_t pos, uint32_t step, float (&sc)[2][4]) {
+                                           Factor f, const Tile& t, int64_t pos, uint32_t step, float (&sc)[2][4]) {
   const uint32_t lane = threadIdx.x & 63;
   i32x4 acc[2][4];
   asm volatile("" ::: "memory");  // the digits are read in every step, not held
@@ -692,7 +722,7 @@ __device__ __forceinline__ void score_step(const Kv8AttnArgs& a, const Codes<NL>
       acc[1][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k.c[1][l], q, acc[1][d], 0, 0, 0);
     }
   }
-  finish_scores(a, acc, k.s, vs, k.has, qmul, t, pos, step, sc);
+  finish_scores(a, acc, k.s, vs, k.has, f, t, pos, step, sc);
 }
 
 template <int NL>
@@ -729,10 +759,9 @@ __device__ __forceinline__ void digits4(const int (&v)[4], int (&w)[4]) {
 }
 
 // A lane's part of its column's query row (dims 64 l + 16 g ..) as digits; the row's
-// largest magnitude decides their unit, which is returned (NaN where the row has a
-// NaN or an infinity).
+// largest magnitude decides their unit.
 template <int NL>
-__device__ __forceinline__ float load_q(const Kv8AttnArgs& a, const float* q, i32x4 (&qd)[4][NL]) {
+__device__ __forceinline__ Factor load_q(const Kv8AttnArgs& a, const float* q, i32x4 (&qd)[4][NL]) {
   const uint32_t g = (threadIdx.x & 63) >> 4, D = a.c.D;
   f32x4 x[NL][4];
   float amax = 0.f;
@@ -770,7 +799,7 @@ __device__ __forceinline__ float load_q(const Kv8AttnArgs& a, const float* q, i3
 #pragma unroll
       for (int d = 0; d < 4; d++) qd[d][l][j] = w[d];
     }
-  return bad ? __builtin_nanf("") : ldexpf(1.f, e - 30);
+  return factor_of(e - 30, bad, a.scale);
 }
 
 // A wave's part of the query row q (dims 64 l + 16 g .. for every fourth l).
@@ -789,10 +818,9 @@ __device__ __forceinline__ void load_row(const float* q, uint32_t D, f32x4 (&x)[
 
 // The tile's query columns as digits in LDS, qd[digit][l][lane] (dims 64 l + 16 g
 // .. of column n); a wave makes every fourth l.  A row's largest magnitude (joined
-// through qm) decides its unit, which is returned (NaN where the row has a NaN or
-// an infinity).
+// through qm) decides its unit.
 template <int NL>
-__device__ __forceinline__ float stage_q(const f32x4 (&x)[(NL + 3) / 4][4], float* qm, i32x4* qd) {
+__device__ __forceinline__ Factor stage_q(const Kv8AttnArgs& a, const f32x4 (&x)[(NL + 3) / 4][4], float* qm, i32x4* qd) {
   constexpr int NS = (NL + 3) / 4;
   const uint32_t lane = threadIdx.x & 63, wave = wave_id(), n = lane & 15;
   float amax = 0.f;
@@ -834,7 +862,7 @@ __device__ __forceinline__ float stage_q(const f32x4 (&x)[(NL + 3) / 4][4], floa
     for (int d = 0; d < 4; d++) qd[(d * NL + l) * 64 + lane] = w[d];
   }
   __syncthreads();
-  return bad ? __builtin_nanf("") : ldexpf(1.f, e - 30);
+  return factor_of(e - 30, bad, a.scale);
 }
 
 // A lane's sums of its column (dims d0 + 16 g + 4 i .. for each i), times by 2^n (in that
@@ -886,12 +914,12 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
     load_codes<NL, FULL, STREAM, true>(a, t, s, pages, 0, &k);
     load_codes<NL, FULL, STREAM, false>(a, t, s, pages, 0, &v);
   }
-  const float qmul = stage_q<NL>(row, lm, qd) * (a.scale * kLog2e);
+  const Factor qf = stage_q<NL>(a, row, lm, qd);
   Run<NL> r;
   clear<NL>(&r);
   for (; s < s1; s += 4) {
     float sc[2][4];
-    score_step<NL>(a, k, v.s, qd, qmul, t, pos, s, sc);
+    score_step<NL>(a, k, v.s, qd, qf, t, pos, s, sc);
     const bool more = s + 4 < s1;
     if (++i == 32 && more) {
       i = 0;
@@ -1050,7 +1078,7 @@ __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
   i32x4 qd[4][NL];
   uint32_t s = s0 + par;
   if (s < s1) load(s);
-  const float qmul = load_q<NL>(a, a.q + row_at(a, t, col), qd) * (a.scale * kLog2e);
+  const Factor qf = load_q<NL>(a, a.q + row_at(a, t, col), qd);
   // the lowest digits are in LDS: the registers hold three of four
   i32x4* q0 = reinterpret_cast<i32x4*>(lds) + 2 * (kPieces + vPieces) + part * NL * 64;
   if (par == 0) {
@@ -1080,7 +1108,7 @@ __device__ __forceinline__ void attend_rows(const Kv8AttnArgs& a) {
             acc[1][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k1, q, acc[1][d], 0, 0, 0);
           }
         }
-        finish_scores(a, acc, ks, vs, has, qmul, mine, pos, s, sc);
+        finish_scores(a, acc, ks, vs, has, qf, mine, pos, s, sc);
       }
       f16x8 x[4];  // the values' operands, one l ahead
 #pragma unroll

@@ -132,6 +132,40 @@ def test_parts_with_units_of_their_own(gpu, drop, small, large):
     check(run_attn(gpu, dev, rows, past, tables, q, scale, 0), want, bound)
 
 
+@pytest.mark.parametrize("size,scale_k,scale", [(1e-36, 2.0 ** 112, 1.0), (1e-40, 2.0 ** 125, 1.0), (1e-30, 2.0 ** 60, 1e11),
+                                                (1e30, 2.0 ** -104, 1.0), (1e25, 2.0 ** -126, 1e12), (1e-30, 2.0 ** 126, 1e-9)])
+@RUNS
+def test_queries_and_keys_of_sizes_far_apart(gpu, run, size, scale_k, scale):
+    # scores of ordinary size, from factors at the ends of the range of f32
+    nq, H, D, page = 4, 2, 64, 16
+    rng = np.random.default_rng(int(np.log2(scale_k)) + 300)
+    cache = ref.Cache(12, page, H, D, rng)
+    cache.scales[0][:] = scale_k * 2.0 ** -rng.integers(0, 3, cache.scales[0].shape)
+    cache.scales[0][7], cache.codes[0][7] = 0, 0
+    dev = ref.Device(gpu, cache)
+    tables = np.arange(12, dtype=np.uint32)[None]
+    q = (rng.standard_normal((2, nq, D)) * size).astype(np.float32)
+    unit = size * scale_k * scale
+    scale = np.float32(scale * min(1.0, 0.01 / unit))  # (scores of a few units)
+    want, bound = attention(cache, [2], [150], tables, q, float(scale))
+    check(run(gpu, dev, [2], [150], tables, q, float(scale), 0), want, bound)
+
+
+@RUNS
+def test_rows_of_sizes_far_apart_in_one_tile(gpu, run):
+    # the first row's scores are ordinary under key scales of 2^100, the second's under those of 2^-40
+    nq, H, D, page = 4, 2, 64, 16
+    rng = np.random.default_rng(77)
+    cache = ref.Cache(12, page, H, D, rng)
+    for row, scale_k in enumerate((2.0 ** 100, 2.0 ** -40)):
+        cache.scales[0][:] = scale_k
+        dev = ref.Device(gpu, cache)
+        q = rng.standard_normal((2, nq, D)).astype(np.float32) * np.array([[[1e-33]], [[1e9]]], np.float32)
+        want, bound = attention(cache, [2], [150], np.arange(12, dtype=np.uint32)[None], q, 1.0, only={row})
+        got = run(gpu, dev, [2], [150], np.arange(12, dtype=np.uint32)[None], q, 1.0, 0)
+        check(got, want, bound, [row])
+
+
 @pytest.mark.parametrize("size", [1.0, 1e9, 1e30])
 def test_parts_of_scores_past_all_units(gpu, size):
     # equal scores of any size are an average of the values, also of values near f32's end
