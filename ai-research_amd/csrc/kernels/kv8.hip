@@ -659,7 +659,7 @@ struct Factor {
 // Of digits in units of 2^e (odd: of a row with a NaN or an infinity).  Queries so small that their
 // factor is below f32's range (x < -125) have scores that count only under scales far above 1, and
 // lend that range to them, as far as the wave's largest queries can do without scales below
-// 2^(lift - 126).
+// 2^(lift - 126).  (The test for it costs prompts up to 1%.)
 __device__ __forceinline__ Factor factor_of(int e, bool odd, float scale) {
   const float c = scale * kLog2e;
   const int x = e + (int)((__float_as_uint(c) >> 23) & 255u) - 127;
@@ -999,7 +999,7 @@ __device__ __forceinline__ void attend(const Kv8AttnArgs& a) {
 // over the CUs.  The codes of a step come through LDS once for its two waves, the values'
 // already as f16, whose conversion is as much vector work as the softmax; the next
 // step's are on their way to registers meanwhile.  (A prompt of 2000 tokens, 16 heads of
-// 256 over 8 key heads: 95 us, 66 GFLOP made, the matrix cores busy for 32% of it, the
+// 256 over 8 key heads: 97 us, 66 GFLOP made, the matrix cores busy for 32% of it, the
 // vector units for 50%.  64 columns a workgroup took 3% less, but 13 - 20% more for prompts of
 // 350 - 650 tokens.)
 // grid (tiles * kv heads, 1, sequences), the tiles that see most first; the heads in
